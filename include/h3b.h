@@ -196,6 +196,51 @@ H3B_API int h3b_fp8_gemm_gate(const void* a, int64_t lda, const void* w, int64_t
                               int64_t M, int64_t N, int64_t K, h3b_stream_t stream);
 
 /* ---------------------------------------------------------------------------------------------------------------
+ * block-scaled FP8: one fp32 scale per 128 values of a row (activations) or per 128 x 128 tile (weights), the format of
+ * block-quantised checkpoints.  No reference counterpart: the reference quantises per token and per output channel
+ * (h3_tp2/fp8_quant_fuse.py:4-13); the scale and the rounding are the same, taken over a block.
+ * ------------------------------------------------------------------------------------------------------------- */
+
+/* x [rows, cols] bf16 (row stride stride_x) -> q [rows, cols] e4m3 contiguous and scale[r * scale_row + j * scale_block]
+ * f32 for each block j of 128 columns (the last one may be short): amax = max |x| over the block (NaN propagates), scale =
+ * max(amax / 448, 1/(448*512)), q = e4m3_rn(clamp(x * (1/scale), +-448)). */
+H3B_API int h3b_quant_blocks_e4m3(const void* x, int64_t rows, int64_t cols, int64_t stride_x, void* q, float* scale,
+                                  int64_t scale_row, int64_t scale_block, int32_t div_mode, h3b_stream_t stream);
+
+/* x [rows, 2d] bf16 (gate columns, then up columns): the block quant of h = gate / (1 + exp(-gate)) * up, with h in fp32
+ * (h is not rounded to bf16 on the way, unlike h3b_silu_mul_quant_e4m3).  q [rows, d], scales as above. */
+H3B_API int h3b_silu_mul_quant_blocks_e4m3(const void* x, int64_t rows, int64_t d, int64_t stride_x, void* q,
+                                           float* scale, int64_t scale_row, int64_t scale_block, int32_t div_mode,
+                                           h3b_stream_t stream);
+
+/* w [experts, n, k] bf16 (strides stride_e, stride_n, 1; one matrix: experts = 1) -> q [experts, n, k] e4m3 and
+ * scale [experts, ceil(n/128), ceil(k/128)] f32, both contiguous: one scale per 128 x 128 tile. */
+H3B_API int h3b_quant_weight_blocks_e4m3(const void* w, int64_t experts, int64_t n, int64_t k, int64_t stride_e,
+                                         int64_t stride_n, void* q, float* scale, int32_t div_mode,
+                                         h3b_stream_t stream);
+
+/* y[m, n] = out(sum over blocks j of 128 values of K: sa[m, j] * sb[n / 128, j] * (a[m, block j] . w[n, block j])
+ * + bias[n]): each block's product is summed on the tensor cores, the scaled blocks in f32, one rounding to out_dtype.
+ *   a [M, K] e4m3 (row stride lda), w [N, K] e4m3 (row stride ldw), sa[m * sa_row + j * sa_block], sb[(n / 128) * sb_row +
+ *   j * sb_block] f32, bias [N] bf16 or NULL, y [M, N] (row stride ldy >= N, any alignment).
+ * Requirements: K % 16 == 0, lda / ldw multiples of 16, a / w 16-byte aligned; any M and N. */
+H3B_API int h3b_fp8_gemm_blocks(const void* a, int64_t lda, const void* w, int64_t ldw, const float* sa, int64_t sa_row,
+                                int64_t sa_block, const float* sb, int64_t sb_row, int64_t sb_block, const void* bias,
+                                void* y, int64_t ldy, int64_t M, int64_t N, int64_t K, int32_t out_dtype,
+                                h3b_stream_t stream);
+
+/* The same product grouped by expert: rows offsets[e] .. offsets[e+1] - 1 of a (and y) use w[e] (expert stride w_expert,
+ * a multiple of 16) and sb[e] (expert stride sb_expert).  offsets: experts + 1 device integers (offsets_i64 != 0: int64,
+ * else int32), non-decreasing, within [0, rows]; groups may be empty, and rows before the first or behind the last
+ * bound are neither used nor written.  A group whose bounds break this is skipped and H3B_EINVAL recorded in the device
+ * status word.  The sizes are read on the device only. */
+H3B_API int h3b_fp8_gemm_grouped(const void* a, int64_t lda, const void* w, int64_t w_expert, int64_t ldw,
+                                 const float* sa, int64_t sa_row, int64_t sa_block, const float* sb, int64_t sb_expert,
+                                 int64_t sb_row, int64_t sb_block, const void* offsets, int32_t offsets_i64, void* y,
+                                 int64_t ldy, int64_t rows, int64_t experts, int64_t N, int64_t K, int32_t out_dtype,
+                                 h3b_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------------------------------
  * attention (tcgen05 flash attention, non-causal, head_dim 128)
  * ------------------------------------------------------------------------------------------------------------- */
 

@@ -1,0 +1,825 @@
+// Block-scaled FP8 products on the 5th-generation tensor cores:
+//   y[m, n] = out( sum_j sa[m, j] * sb[n / 128, j] * sum_{k in block j} a[m, k] * w[n, k] )  (+ bias[n])
+// with e4m3 operands and one fp32 scale per row of a and 128 values of K, and per 128 x 128 tile of w; dense, or grouped
+// by expert (rows offsets[e] .. offsets[e+1] of a use w[e], read on the device: no host copy of the sizes).
+//
+// The scales change every 128 values of K, so the tensor core's accumulator holds one block's product only: each
+// K step of 128 is its own accumulator in TMEM, and the epilogue warps add it, scaled, to fp32 running sums in
+// registers while the next step's MMAs fill the other TMEM buffer.  Both forms below are that loop:
+//
+//   wide    (many rows): CTA pairs with 2-SM MMAs over 256 rows x 256 columns.  Thread = output row, so sa * sb is one
+//           scalar per thread and step and the promotion costs one FMA per element: 8 warps x 128 FMAs per 512 tensor
+//           cycles.  128 running sums per thread, two 256-column TMEM buffers.
+//   narrow  (few rows): the operands swapped, D^T = w a^T: 128 weight rows x NT tokens (NT = 16 .. 128) per CTA, so that
+//           a tile streams the weight once with no tensor work on absent rows.  K is split over a cluster of CTAs that
+//           add their sums through distributed shared memory in a fixed order (the result does not depend on timing).
+//
+// Every wait is bounded (common.cuh); no TMA multicast.
+#include <atomic>
+
+#include "common.cuh"
+
+namespace h3b {
+namespace {
+
+constexpr int BLK = 128;
+constexpr int MAX_DEVICES = 64;
+
+struct Params {
+  int64_t T, N;       // rows of a, rows of w (of one expert)
+  int num_kb;         // 128-value blocks of K
+  int num_nb;         // column tiles (256 wide, or 128 weight rows narrow)
+  int experts;        // groups; dense: 1 without offsets
+  const void* offsets;
+  int off64;          // offsets are int64 (else int32)
+  const float* sa;
+  int64_t sa_row, sa_blk;
+  const float* sb;
+  int64_t sb_exp, sb_row, sb_blk;
+  const __nv_bfloat16* bias;
+  uint16_t* y;
+  int64_t ldy;
+  int out_f16;
+  int tma_out;        // wide: whole slices leave through TMA stores
+  int vec_out;        // y rows are 16-byte granular
+  WaitCtl wc;
+};
+
+__device__ __forceinline__ int64_t group_bound(const Params& p, int e) {
+  return p.off64 ? __ldg(static_cast<const int64_t*>(p.offsets) + e)
+                 : static_cast<int64_t>(__ldg(static_cast<const int32_t*>(p.offsets) + e));
+}
+
+__device__ __forceinline__ uint16_t to_out(float v, int f16) {
+  return f16 ? __half_as_ushort(__float2half_rn(v)) : __bfloat16_as_ushort(__float2bfloat16_rn(v));
+}
+__device__ __forceinline__ uint32_t to_out2(float lo, float hi, int f16) {
+  return static_cast<uint32_t>(to_out(lo, f16)) | (static_cast<uint32_t>(to_out(hi, f16)) << 16);
+}
+
+// Walk over the row tiles of the groups in order.  `before`: tiles of the experts below e0.  find() places tile t
+// (non-decreasing over calls) with the whole warp: 32 experts' bounds per step and a shuffle scan.  A group whose bounds
+// are not 0 <= lo <= hi <= T has no tiles, and `bad` is set (recorded by the caller once its cluster is done, so that
+// the CTAs of a cluster never disagree on whether to start).
+template <int ROWS>
+struct Walk {
+  int e0 = 0;
+  int64_t before = 0;
+  bool bad = false;
+  int e;               // the tile found: expert, its rows [lo, hi), row blocks and the tile's index within the expert
+  int64_t lo, hi;
+  int blocks, r;
+  __device__ bool find(const Params& p, int64_t t, int per_block) {
+    const int lane = threadIdx.x & 31;
+    while (e0 < p.experts) {
+      int64_t l = 0, h = 0;
+      if (e0 + lane < p.experts) {
+        if (p.offsets == nullptr) {
+          h = p.T;
+        } else {
+          l = group_bound(p, e0 + lane);
+          h = group_bound(p, e0 + lane + 1);
+          if (l < 0 || h < l || h > p.T) {
+            l = h = 0;
+            bad = true;
+          }
+        }
+      }
+      const int mine = static_cast<int>((h - l + ROWS - 1) / ROWS);
+      int64_t sum = static_cast<int64_t>(mine) * per_block;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t up = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += up;
+      }
+      const int64_t total = __shfl_sync(0xffffffffu, sum, 31);
+      if (t < before + total) {
+        const int64_t rel = t - before;
+        const int src = __ffs(__ballot_sync(0xffffffffu, sum > rel)) - 1;
+        e = e0 + src;
+        lo = __shfl_sync(0xffffffffu, l, src);
+        hi = __shfl_sync(0xffffffffu, h, src);
+        blocks = __shfl_sync(0xffffffffu, mine, src);
+        r = static_cast<int>(rel - (__shfl_sync(0xffffffffu, sum, src) - static_cast<int64_t>(blocks) * per_block));
+        return true;
+      }
+      before += total;
+      e0 += 32;
+    }
+    return false;
+  }
+};
+
+// whether this cluster starts: the status word as its first CTA read it (so that all its CTAs take the same way).
+// Call between two cluster-wide barriers that keep the first CTA's shared memory alive.
+__device__ __forceinline__ bool cluster_flag(uint32_t flag_smem) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(mapa_shared(flag_smem, 0)) : "memory");
+  return v != 0;
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// wide: CTA pairs, 256 x 256 tiles, running sums in registers
+// ---------------------------------------------------------------------------------------------------------------
+namespace wide {
+
+constexpr int BM = 128, BN = 256, STAGES = 6;
+constexpr int STAGE_BYTES = 2 * BM * BLK;           // this CTA's 128 rows of a and 128 rows of w, 128 bytes each
+constexpr int EPI_WARPS = 8, THREADS = 64 + 32 * EPI_WARPS;
+constexpr int WARP_STAGING = 32 * 128;              // 32 rows x 64 columns of 16-bit output
+constexpr int SMEM = STAGES * STAGE_BYTES + 1024 + 1024 + EPI_WARPS * WARP_STAGING;
+static_assert(SMEM <= 232448, "shared memory");
+constexpr uint32_t IDESC = idesc_make(FMT_E4M3, FMT_E4M3, 0, 2 * BM, BN);
+// row blocks (256 rows) that share a column block's w tile in L2, as in the per-token product
+constexpr int GROUP_M = 16;
+
+// tile r of a group of `blocks` row blocks -> (row block, column block)
+__device__ __forceinline__ void coords(int r, int blocks, int num_nb, int& mb, int& nb) {
+  const int in_group = GROUP_M * num_nb;
+  const int g = r / in_group, first = g * GROUP_M;
+  const int size = min(blocks - first, GROUP_M);
+  const int q = r - g * in_group;
+  mb = first + q % size;
+  nb = q / size;
+}
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+    kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
+           const __grid_constant__ CUtensorMap tmY, const __grid_constant__ Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE_BYTES);
+  // bars: full[STAGES], empty[STAGES], tfull[2], tempty[2], done; then the TMEM address and the start flag
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 5);
+  uint32_t* start_flag = tmem_slot + 1;
+  uint8_t* staging = smem + STAGES * STAGE_BYTES + 1024;
+  const uint32_t smem0 = smem_u32(smem), bar0 = smem_u32(bars);
+  auto full_bar = [&](int s) { return bar0 + 8u * s; };
+  auto empty_bar = [&](int s) { return bar0 + 8u * (STAGES + s); };
+  auto tfull_bar = [&](int b) { return bar0 + 8u * (2 * STAGES + b); };
+  auto tempty_bar = [&](int b) { return bar0 + 8u * (2 * STAGES + 2 + b); };
+  const uint32_t done_bar = bar0 + 8u * (2 * STAGES + 4);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int crank = static_cast<int>(cluster_ctarank());  // 0: the pair's leader (issues the MMAs)
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(tfull_bar(b), 1);
+      mbar_init(tempty_bar(b), 2 * EPI_WARPS);  // one arrival per epilogue warp of both CTAs, on the leader's
+    }
+    mbar_init(done_bar, 1);
+    fence_mbar_init();
+    *start_flag = status_bad(p.wc) ? 0u : 1u;
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmW);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(smem_u32(tmem_slot), 512);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  const bool start = cluster_flag(smem_u32(start_flag));
+  const int first_tile = static_cast<int>(cluster_id_x()), tile_step = static_cast<int>(cluster_count_x());
+  Walk<2 * BM> walk;
+
+  if (start) {
+    if (warp == 0) {
+      // ---------------- TMA producer (both CTAs; stages complete on the leader's full barrier) ----------------
+      const uint32_t lead_full0 = mapa_shared(full_bar(0), 0);
+      int stage = 0;
+      uint32_t phase = 0;
+      uint32_t used = 0, last = 0;  // per stage: loaded at all, parity of its last load
+      bool ok = true;
+      for (int64_t t = first_tile; ok && walk.find(p, t, p.num_nb); t += tile_step) {
+        int mb, nb;
+        coords(walk.r, walk.blocks, p.num_nb, mb, nb);
+        const int arow = static_cast<int>(walk.lo) + (2 * mb + crank) * BM;
+        const int wrow = nb * BN + crank * BM;
+        if (lane == 0) {
+          for (int kb = 0; kb < p.num_kb; ++kb) {
+            if (!mbar_wait(empty_bar(stage), phase ^ 1u, p.wc)) {
+              ok = false;
+              break;
+            }
+            const uint32_t sA = smem0 + stage * STAGE_BYTES;
+            if (crank == 0) mbar_arrive_expect_tx(full_bar(stage), 2 * STAGE_BYTES);
+            tma_load_2d_pair(sA, &tmA, lead_full0 + 8u * stage, kb * BLK, arow);
+            tma_load_3d_pair(sA + BM * BLK, &tmW, lead_full0 + 8u * stage, kb * BLK, wrow, walk.e);
+            used |= 1u << stage;
+            last = (last & ~(1u << stage)) | (phase << stage);
+            if (++stage == STAGES) {
+              stage = 0;
+              phase ^= 1u;
+            }
+          }
+        }
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+      }
+      // drain: no TMA write may be in flight into shared memory that the CTA is about to give up.  The leader sees
+      // both CTAs' bytes on its full barriers; the partner's last load of a stage has landed once the leader's MMAs
+      // consumed it.
+      if (lane == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+          if (!(used >> s & 1u)) continue;
+          const uint32_t bar = crank == 0 ? full_bar(s) : empty_bar(s), par = last >> s & 1u;
+          const uint64_t t0 = globaltimer();
+          while (!mbar_try_wait(bar, par) && globaltimer() - t0 < p.wc.timeout) {
+          }
+        }
+      }
+    } else if (warp == 1) {
+      if (crank == 0) {
+        // ---------------- MMA issuer (the leader only): one accumulator per 128-value step of K ----------------
+        int stage = 0;
+        uint32_t phase = 0;
+        uint32_t it = 0;  // steps so far: TMEM buffer it & 1
+        bool ok = true;
+        for (int64_t t = first_tile; ok && walk.find(p, t, p.num_nb); t += tile_step) {
+          if (lane == 0) {
+            for (int kb = 0; kb < p.num_kb; ++kb, ++it) {
+              const int b = it & 1;
+              if (!mbar_wait(tempty_bar(b), ((it >> 1) & 1u) ^ 1u, p.wc) || !mbar_wait(full_bar(stage), phase, p.wc)) {
+                ok = false;
+                break;
+              }
+              tc_fence_after();
+              const uint32_t sA = smem0 + stage * STAGE_BYTES;
+              const uint64_t adesc = sdesc_sw128(sA, 16, 1024), bdesc = sdesc_sw128(sA + BM * BLK, 16, 1024);
+#pragma unroll
+              for (int kk = 0; kk < BLK / 32; ++kk)
+                umma_f8_ss_pair(tmem_base + static_cast<uint32_t>(b * BN), adesc + 2u * kk, bdesc + 2u * kk, IDESC, kk != 0);
+              umma_commit_pair_mc(tfull_bar(b), 3);
+              umma_commit_pair_mc(empty_bar(stage), 3);
+              if (++stage == STAGES) {
+                stage = 0;
+                phase ^= 1u;
+              }
+            }
+          }
+          ok = __shfl_sync(0xffffffffu, ok, 0);
+        }
+        if (lane == 0) {  // every issued MMA completes before TMEM is released
+          umma_commit_pair(done_bar);
+          const uint64_t t0 = globaltimer();
+          while (!mbar_try_wait(done_bar, 0) && globaltimer() - t0 < p.wc.timeout) {
+          }
+        }
+      }
+    } else {
+      // ---------------- epilogue warps: 32 rows x 128 columns of running sums each ----------------
+      const int sub = warp & 3, half = (warp - 2) >> 2;
+      const uint32_t tmine = tmem_base + (static_cast<uint32_t>(sub * 32) << 16) + static_cast<uint32_t>(half * 128);
+      const uint32_t lead_tempty0 = mapa_shared(tempty_bar(0), 0);
+      uint4* stg = reinterpret_cast<uint4*>(staging + (warp - 2) * WARP_STAGING);
+      uint32_t it = 0;
+      bool ok = true;
+      for (int64_t t = first_tile; ok && walk.find(p, t, p.num_nb); t += tile_step) {
+        int mb, nb;
+        coords(walk.r, walk.blocks, p.num_nb, mb, nb);
+        const int64_t m0 = walk.lo + (2 * mb + crank) * BM + sub * 32;  // the warp's first row
+        const int64_t n0 = static_cast<int64_t>(nb) * BN + half * 128;  // and first column
+        const bool row_ok = m0 + lane < walk.hi, col_ok = n0 < p.N;
+        const float* sap = p.sa + (row_ok ? m0 + lane : walk.lo) * p.sa_row;
+        const float* sbp = p.sb + walk.e * p.sb_exp + (col_ok ? n0 / BLK : 0) * p.sb_row;
+        float acc[128];
+#pragma unroll
+        for (int i = 0; i < 128; ++i) acc[i] = 0.0f;
+        // the scales of the next two steps are on their way while a step is added
+        float sa0 = __ldg(sap), sb0 = __ldg(sbp);
+        float sa1 = p.num_kb > 1 ? __ldg(sap + p.sa_blk) : 0.0f, sb1 = p.num_kb > 1 ? __ldg(sbp + p.sb_blk) : 0.0f;
+#pragma unroll 1
+        for (int kb = 0; kb < p.num_kb; ++kb, ++it) {
+          const float s = sa0 * sb0;
+          sa0 = sa1;
+          sb0 = sb1;
+          if (kb + 2 < p.num_kb) {
+            sa1 = __ldg(sap + (kb + 2) * p.sa_blk);
+            sb1 = __ldg(sbp + (kb + 2) * p.sb_blk);
+          }
+          const int b = it & 1;
+          if (!__all_sync(0xffffffffu, mbar_wait(tfull_bar(b), (it >> 1) & 1u, p.wc))) {
+            ok = false;  // for the whole warp: the TMEM loads below need all of it
+            break;
+          }
+          tc_fence_after();
+          const uint32_t tcur = tmine + static_cast<uint32_t>(b * BN);
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            uint32_t r[16];
+            tmem_ld16(tcur + 16 * c, r);
+            tmem_ld_wait();
+            reg_fence(r);
+            if (c == 7) {  // this warp has read the buffer: the next step's MMAs may overwrite it
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive_cluster_relaxed(lead_tempty0 + 8u * b);
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[16 * c + i] = fmaf(__uint_as_float(r[i]), s, acc[16 * c + i]);
+          }
+        }
+        if (!ok) break;
+        if (p.bias != nullptr) {
+#pragma unroll
+          for (int i = 0; i < 128; ++i)
+            if (n0 + i < p.N) acc[i] += __bfloat162float(p.bias[n0 + i]);
+        }
+        // two halves of 64 columns through the warp's staging: 32 rows x 128 bytes in the 128-byte swizzle
+        const bool whole = p.tma_out && m0 + 32 <= walk.hi;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (p.tma_out && lane == 0) bulk_wait_read0();
+          __syncwarp();
+#pragma unroll
+          for (int g = 0; g < 8; ++g) {
+            const float* v = acc + 64 * h + 8 * g;
+            stg[lane * 8 + (g ^ (lane & 7))] = make_uint4(to_out2(v[0], v[1], p.out_f16), to_out2(v[2], v[3], p.out_f16),
+                                                          to_out2(v[4], v[5], p.out_f16), to_out2(v[6], v[7], p.out_f16));
+          }
+          const int64_t nh = n0 + 64 * h;
+          if (whole) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0 && nh < p.N) {
+              tma_store_2d(&tmY, smem_u32(stg), static_cast<int32_t>(nh), static_cast<int32_t>(m0));
+              bulk_commit();
+            }
+          } else {
+            __syncwarp();
+#pragma unroll 1
+            for (int i = lane; i < 32 * 8; i += 32) {
+              const int r = i >> 3, g = i & 7;
+              const int64_t m = m0 + r, n = nh + 8 * g;
+              if (m >= walk.hi || n >= p.N) continue;
+              const uint4 val = stg[r * 8 + (g ^ (r & 7))];
+              uint16_t* dst = p.y + m * p.ldy + n;
+              if (p.vec_out && n + 8 <= p.N) {
+                *reinterpret_cast<uint4*>(dst) = val;
+              } else {
+                const uint32_t w[4] = {val.x, val.y, val.z, val.w};
+#pragma unroll
+                for (int e2 = 0; e2 < 8; ++e2)
+                  if (n + e2 < p.N) dst[e2] = static_cast<uint16_t>(w[e2 >> 1] >> (16 * (e2 & 1)));
+              }
+            }
+            __syncwarp();
+          }
+        }
+      }
+      if (p.tma_out && lane == 0) bulk_wait_all0();  // this warp's TMA stores are complete before the CTA leaves
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  cluster_sync();  // neither CTA leaves (or frees the pair's TMEM) while the other may still signal it
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc_pair(tmem_base, 512);
+  if (walk.bad) record_status(p.wc, H3B_EINVAL);
+}
+
+}  // namespace wide
+
+// ---------------------------------------------------------------------------------------------------------------
+// narrow: 128 weight rows x NT tokens per CTA, K split over the cluster
+// ---------------------------------------------------------------------------------------------------------------
+namespace narrow {
+
+constexpr int THREADS = 192;    // producer, MMA issuer, 4 epilogue warps
+constexpr int CHUNK = 16;       // K steps whose scales are staged together
+constexpr int MAX_SPLIT = 8;
+
+__host__ __device__ constexpr int stage_bytes(int nt) { return (BLK + nt) * BLK; }
+__host__ __device__ constexpr int stages(int nt) { return nt >= 128 ? 3 : 4; }
+// TMEM buffers of NT columns: 4 (a step of few tokens is short, so more of them are in flight), 2 for wide tiles
+__host__ __device__ constexpr int buffers(int nt) { return nt >= 64 ? 2 : 4; }
+// ring (reused for the sums that the cluster adds: NT x 128 fp32), barriers, two chunks of scales, alignment slack
+__host__ __device__ constexpr int smem(int nt) {
+  return stages(nt) * stage_bytes(nt) + 256 + 2 * CHUNK * nt * 4 + 1024;
+}
+// TMEM is never oversubscribed (a CTA that waited for TMEM while its cluster waits for it could wait forever): at most
+// 232448 / smem CTAs fit on an SM, and that many allocations fit in its 512 columns
+__host__ __device__ constexpr bool tmem_fits(int nt) { return (233472 / (smem(nt) + 1024)) * (buffers(nt) * nt) <= 512; }
+static_assert(tmem_fits(16) && tmem_fits(32) && tmem_fits(64) && tmem_fits(128), "TMEM columns");
+static_assert(stages(128) * stage_bytes(128) >= 128 * BLK * 4 && stages(16) * stage_bytes(16) >= 16 * BLK * 4 &&
+              stages(64) * stage_bytes(64) >= 64 * BLK * 4, "the ring holds the sums");
+
+template <int NT>
+__global__ void __launch_bounds__(THREADS, 2) kernel(const __grid_constant__ CUtensorMap tmA,
+                                                     const __grid_constant__ CUtensorMap tmW,
+                                                     const __grid_constant__ Params p) {
+  constexpr int STAGES = stages(NT), STAGE_BYTES = stage_bytes(NT), NBUF = buffers(NT);
+  constexpr uint32_t TMEM_COLS = NBUF * NT, IDESC = idesc_make(FMT_E4M3, FMT_E4M3, 0, 128, NT);
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE_BYTES);
+  // bars: full[STAGES], empty[STAGES], tfull[NBUF], tempty[NBUF], done; then the TMEM address and the start flag
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 2 * NBUF + 1);
+  uint32_t* start_flag = tmem_slot + 1;
+  float* scales = reinterpret_cast<float*>(smem + STAGES * STAGE_BYTES + 256);  // [2][CHUNK][NT]
+  float* sums = reinterpret_cast<float*>(smem);                                 // [NT][128] once the ring is idle
+  static_assert(8 * (2 * STAGES + 2 * NBUF + 1) + 8 <= 256, "barrier area");
+  const uint32_t smem0 = smem_u32(smem), bar0 = smem_u32(bars);
+  auto full_bar = [&](int s) { return bar0 + 8u * s; };
+  auto empty_bar = [&](int s) { return bar0 + 8u * (STAGES + s); };
+  auto tfull_bar = [&](int b) { return bar0 + 8u * (2 * STAGES + b); };
+  auto tempty_bar = [&](int b) { return bar0 + 8u * (2 * STAGES + NBUF + b); };
+  const uint32_t done_bar = bar0 + 8u * (2 * STAGES + 2 * NBUF);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int split = static_cast<int>(gridDim.x) / p.num_nb;  // CTAs of the cluster: they share blockIdx.x / split
+  const int crank = static_cast<int>(blockIdx.x) % split, nb = static_cast<int>(blockIdx.x) / split;
+  Walk<NT> walk;
+  const bool found = walk.find(p, blockIdx.y, 1);  // the same for every CTA of the cluster
+  if (!found) {
+    if (walk.bad) record_status(p.wc, H3B_EINVAL);
+    return;
+  }
+  const int64_t t0 = walk.lo + static_cast<int64_t>(walk.r) * NT;  // the tile's first row of a
+  const int kb0 = static_cast<int>(static_cast<int64_t>(p.num_kb) * crank / split);
+  const int kb1 = static_cast<int>(static_cast<int64_t>(p.num_kb) * (crank + 1) / split);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    for (int b = 0; b < NBUF; ++b) {
+      mbar_init(tfull_bar(b), 1);
+      mbar_init(tempty_bar(b), 4);
+    }
+    mbar_init(done_bar, 1);
+    fence_mbar_init();
+    *start_flag = status_bad(p.wc) ? 0u : 1u;
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_slot), TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  const bool start = cluster_flag(smem_u32(start_flag));
+  float acc[NT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) acc[i] = 0.0f;
+
+  if (start) {
+    if (warp == 0) {
+      if (lane == 0) {
+        uint32_t used = 0, last = 0;
+        int stage = 0;
+        uint32_t phase = 0;
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!mbar_wait(empty_bar(stage), phase ^ 1u, p.wc)) break;
+          const uint32_t sW = smem0 + stage * STAGE_BYTES;
+          mbar_arrive_expect_tx(full_bar(stage), STAGE_BYTES);
+          tma_load_3d(sW, &tmW, full_bar(stage), kb * BLK, nb * BLK, walk.e);
+          tma_load_2d(sW + BLK * BLK, &tmA, full_bar(stage), kb * BLK, static_cast<int32_t>(t0));
+          used |= 1u << stage;
+          last = (last & ~(1u << stage)) | (phase << stage);
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        for (int s = 0; s < STAGES; ++s) {  // no TMA write in flight when the ring is given up
+          if (!(used >> s & 1u)) continue;
+          const uint64_t c0 = globaltimer();
+          while (!mbar_try_wait(full_bar(s), last >> s & 1u) && globaltimer() - c0 < p.wc.timeout) {
+          }
+        }
+      }
+    } else if (warp == 1) {
+      if (lane == 0) {
+        int stage = 0;
+        uint32_t phase = 0, it = 0;
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+          const int b = it % NBUF;
+          if (!mbar_wait(tempty_bar(b), ((it / NBUF) & 1u) ^ 1u, p.wc) || !mbar_wait(full_bar(stage), phase, p.wc)) break;
+          tc_fence_after();
+          const uint32_t sW = smem0 + stage * STAGE_BYTES;
+          const uint64_t wdesc = sdesc_sw128(sW, 16, 1024), adesc = sdesc_sw128(sW + BLK * BLK, 16, 1024);
+#pragma unroll
+          for (int kk = 0; kk < BLK / 32; ++kk)
+            umma_f8_ss(tmem_base + static_cast<uint32_t>(b * NT), wdesc + 2u * kk, adesc + 2u * kk, IDESC, kk != 0);
+          umma_commit(tfull_bar(b));
+          umma_commit(empty_bar(stage));
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        umma_commit(done_bar);
+        const uint64_t c0 = globaltimer();
+        while (!mbar_try_wait(done_bar, 0) && globaltimer() - c0 < p.wc.timeout) {
+        }
+      }
+    } else {
+      // ---------------- epilogue: thread = weight row, NT running sums ----------------
+      const int sub = warp & 3, tid = threadIdx.x - 64;
+      const uint32_t tmine = tmem_base + (static_cast<uint32_t>(sub * 32) << 16);
+      const float* sbp = p.sb + walk.e * p.sb_exp + nb * p.sb_row;
+      // sa * sb of a chunk of steps for the tile's tokens; thread tid holds values tid, tid + 128, ... of [CHUNK][NT]
+      constexpr int PER = CHUNK * NT / 128;
+      float next[PER];
+      auto fetch = [&](int kb) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          const int v = tid + 128 * i, k = kb + v / NT, tok = v % NT;
+          next[i] = (k < kb1 && t0 + tok < walk.hi)
+                        ? __ldg(p.sa + (t0 + tok) * p.sa_row + k * p.sa_blk) * __ldg(sbp + k * p.sb_blk)
+                        : 0.0f;
+        }
+      };
+      fetch(kb0);
+      uint32_t it = 0;
+      bool ok = true;
+      // every thread of the 128 takes the barrier of each chunk, also after a wait that gave up
+      for (int c0 = kb0; c0 < kb1; c0 += CHUNK) {
+        float* sc = scales + (((c0 - kb0) / CHUNK) & 1) * CHUNK * NT;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) sc[tid + 128 * i] = next[i];
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        if (c0 + CHUNK < kb1) fetch(c0 + CHUNK);
+        const int c1 = min(c0 + CHUNK, kb1);
+#pragma unroll 1
+        for (int kb = c0; kb < c1; ++kb, ++it) {
+          const int b = it % NBUF;
+          ok = __all_sync(0xffffffffu, ok && mbar_wait(tfull_bar(b), (it / NBUF) & 1u, p.wc));
+          if (!ok) break;
+          tc_fence_after();
+          const float* s = sc + (kb - c0) * NT;
+          constexpr int W = NT == 32 || NT == 64 ? 32 : 16;
+#pragma unroll
+          for (int c = 0; c < NT / W; ++c) {
+            uint32_t r[W];
+            if constexpr (W == 16)
+              tmem_ld16(tmine + static_cast<uint32_t>(b * NT + c * 16), r);
+            else
+              tmem_ld32(tmine + static_cast<uint32_t>(b * NT + c * 32), r);
+            tmem_ld_wait();
+            reg_fence(r);
+            if (c == NT / W - 1) {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(tempty_bar(b));
+            }
+#pragma unroll
+            for (int i = 0; i < W; i += 4) {
+              const float4 f = *reinterpret_cast<const float4*>(s + c * W + i);
+              acc[c * W + i] = fmaf(__uint_as_float(r[i]), f.x, acc[c * W + i]);
+              acc[c * W + i + 1] = fmaf(__uint_as_float(r[i + 1]), f.y, acc[c * W + i + 1]);
+              acc[c * W + i + 2] = fmaf(__uint_as_float(r[i + 2]), f.z, acc[c * W + i + 2]);
+              acc[c * W + i + 3] = fmaf(__uint_as_float(r[i + 3]), f.w, acc[c * W + i + 3]);
+            }
+          }
+        }
+      }
+    }
+  }
+  __syncwarp();
+  __syncthreads();  // the ring is idle: every load has landed and every MMA has read it
+  const int64_t n = static_cast<int64_t>(nb) * BLK + (warp & 3) * 32 + lane;
+  const bool epi = warp >= 2;
+  const float bias = epi && p.bias != nullptr && n < p.N ? __bfloat162float(p.bias[n]) : 0.0f;
+  const int tokens = static_cast<int>(walk.hi - t0 < NT ? walk.hi - t0 : NT);
+  if (split == 1) {
+    if (epi && start && n < p.N) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+        if (i < tokens) p.y[(t0 + i) * p.ldy + n] = to_out(acc[i] + bias, p.out_f16);
+    }
+  } else {
+    const int col = (warp & 3) * 32 + lane;
+    if (epi) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i) sums[i * BLK + col] = acc[i];
+    }
+    __syncwarp();
+    cluster_sync();
+    if (epi && start && n < p.N) {
+      // CTA r of the cluster adds and stores tokens r, r + split, ...: the parts in the order of K
+      for (int i = crank; i < tokens; i += split) {
+        float v = 0.0f;
+        for (int q = 0; q < split; ++q) {
+          float part;
+          asm volatile("ld.shared::cluster.f32 %0, [%1];"
+                       : "=f"(part)
+                       : "r"(mapa_shared(smem0 + static_cast<uint32_t>((i * BLK + col) * 4), static_cast<uint32_t>(q)))
+                       : "memory");
+          v += part;
+        }
+        p.y[(t0 + i) * p.ldy + n] = to_out(v + bias, p.out_f16);
+      }
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  cluster_sync();  // the other CTAs have read this CTA's sums (and its start flag)
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem_base, TMEM_COLS);
+  if (walk.bad) record_status(p.wc, H3B_EINVAL);
+}
+
+}  // namespace narrow
+
+// ---------------------------------------------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------------------------------------------
+bool al16(const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15u) == 0; }
+
+int load_map(CUtensorMap* map, const void* base, int64_t K, int64_t rows, int64_t ld, uint32_t box_rows) {
+  const uint64_t dims[2] = {static_cast<uint64_t>(K), static_cast<uint64_t>(rows)};
+  const uint64_t strides[1] = {static_cast<uint64_t>(ld)};
+  const uint32_t box[2] = {BLK, box_rows};
+  return encode_tmap(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+int weight_map(CUtensorMap* map, const void* base, int64_t K, int64_t N, int64_t E, int64_t ldw, int64_t stride_e) {
+  const uint64_t dims[3] = {static_cast<uint64_t>(K), static_cast<uint64_t>(N), static_cast<uint64_t>(E)};
+  const uint64_t strides[2] = {static_cast<uint64_t>(ldw), static_cast<uint64_t>(stride_e)};
+  const uint32_t box[3] = {BLK, BLK, 1};
+  return encode_tmap(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+int launch_wide(Params& p, const CUtensorMap& tmA, const CUtensorMap& tmW, int64_t tiles, int dev, cudaStream_t st) {
+  static std::atomic<int> fit_of[MAX_DEVICES];
+  int fit = fit_of[dev].load(std::memory_order_acquire);
+  if (fit == 0) {
+    cudaError_t e = cudaFuncSetAttribute(wide::kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, wide::SMEM);
+    if (e == cudaSuccess) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(static_cast<unsigned>(num_sms() & ~1), 1, 1);
+      cfg.blockDim = dim3(wide::THREADS, 1, 1);
+      cfg.dynamicSmemBytes = wide::SMEM;
+      e = cudaOccupancyMaxActiveClusters(&fit, wide::kernel, &cfg);
+    }
+    if (e != cudaSuccess) return cuda_fail(e, "fp8_gemm_blocks: shared memory / cluster occupancy");
+    if (fit < 1) return fail(H3B_EUNSUPPORTED, "fp8_gemm_blocks: no CTA pair fits on this device");
+    fit_of[dev].store(fit, std::memory_order_release);
+  }
+  CUtensorMap tmY = tmA;  // a valid map where no TMA store is made
+  p.vec_out = al16(p.y) && p.ldy % 8 == 0;
+  if (p.vec_out) {
+    const uint64_t dims[2] = {static_cast<uint64_t>(p.N), static_cast<uint64_t>(p.T)};
+    const uint64_t strides[1] = {static_cast<uint64_t>(p.ldy) * 2};
+    const uint32_t box[2] = {64, 32};
+    const int rc = encode_tmap(&tmY, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, p.y, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc) return rc;
+    p.tma_out = 1;
+  }
+  const int grid = 2 * static_cast<int>(tiles < fit ? tiles : fit);
+  wide::kernel<<<grid, wide::THREADS, wide::SMEM, st>>>(tmA, tmW, tmY, p);
+  H3B_CHECK_LAUNCH("fp8_gemm_blocks launch");
+  return H3B_OK;
+}
+
+template <int NT>
+int launch_narrow(const Params& p, const CUtensorMap& tmA, const CUtensorMap& tmW, int64_t token_tiles, int split, int dev,
+                  cudaStream_t st) {
+  static std::atomic<int> ready[MAX_DEVICES];
+  if (!ready[dev].load(std::memory_order_acquire)) {
+    const cudaError_t e = cudaFuncSetAttribute(narrow::kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, narrow::smem(NT));
+    if (e != cudaSuccess) return cuda_fail(e, "fp8_gemm_blocks: shared memory");
+    ready[dev].store(1, std::memory_order_release);
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(p.num_nb * split), static_cast<unsigned>(token_tiles), 1);
+  cfg.blockDim = dim3(narrow::THREADS, 1, 1);
+  cfg.dynamicSmemBytes = narrow::smem(NT);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(split);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, narrow::kernel<NT>, tmA, tmW, p);
+  if (e != cudaSuccess) return cuda_fail(e, "fp8_gemm_blocks launch");
+  return H3B_OK;
+}
+
+struct Operands {
+  const void* a;
+  int64_t lda;
+  const void* w;
+  int64_t ldw, w_exp;
+  const float* sa;
+  int64_t sa_row, sa_blk;
+  const float* sb;
+  int64_t sb_exp, sb_row, sb_blk;
+  const void* bias;
+  const void* offsets;
+  int off64;
+  void* y;
+  int64_t ldy;
+  int64_t T, N, K, E;
+  int out_dtype;
+};
+
+int gemm_blocks(const char* what, const Operands& o, cudaStream_t st) {
+  const int64_t most = (1ll << 31) - 1;
+  if (o.T < 0 || o.N <= 0 || o.K <= 0 || o.E <= 0)
+    return fail(H3B_EINVAL, "%s: rows %lld N %lld K %lld experts %lld", what, (long long)o.T, (long long)o.N,
+                (long long)o.K, (long long)o.E);
+  if (o.out_dtype != H3B_OUT_BF16 && o.out_dtype != H3B_OUT_F16) return fail(H3B_EINVAL, "%s: out dtype %d", what, o.out_dtype);
+  if (o.T == 0) return H3B_OK;
+  if (o.a == nullptr || o.w == nullptr || o.sa == nullptr || o.sb == nullptr || o.y == nullptr)
+    return fail(H3B_EINVAL, "%s: null operand", what);
+  if (o.K % 16) return fail(H3B_EUNSUPPORTED, "%s: K %lld must be a multiple of 16", what, (long long)o.K);
+  if (o.lda < o.K || o.ldw < o.K || o.lda % 16 || o.ldw % 16 || o.w_exp % 16 || !al16(o.a) || !al16(o.w))
+    return fail(H3B_EALIGN, "%s: a and w must be 16-byte aligned with strides that are multiples of 16 and at least K", what);
+  if (o.w_exp < 0 || (o.E > 1 && o.w_exp == 0) || o.sa_row < 0 || o.sa_blk < 0 || o.sb_exp < 0 || o.sb_row < 0 || o.sb_blk < 0)
+    return fail(H3B_EINVAL, "%s: negative stride, or a zero one between experts", what);
+  if (o.ldy < o.N) return fail(H3B_EINVAL, "%s: ldy %lld below N", what, (long long)o.ldy);
+  if (o.T > most - 256 || o.N > most - 256 || o.K > most - 256 || o.E > most - 32)
+    return fail(H3B_EUNSUPPORTED, "%s: sizes at or above 2^31", what);
+
+  Params p{};
+  p.T = o.T;
+  p.N = o.N;
+  p.num_kb = static_cast<int>((o.K + BLK - 1) / BLK);
+  p.experts = static_cast<int>(o.E);
+  p.offsets = o.offsets;
+  p.off64 = o.off64;
+  p.sa = o.sa;
+  p.sa_row = o.sa_row;
+  p.sa_blk = o.sa_blk;
+  p.sb = o.sb;
+  p.sb_exp = o.sb_exp;
+  p.sb_row = o.sb_row;
+  p.sb_blk = o.sb_blk;
+  p.bias = static_cast<const __nv_bfloat16*>(o.bias);
+  p.y = static_cast<uint16_t*>(o.y);
+  p.ldy = o.ldy;
+  p.out_f16 = o.out_dtype == H3B_OUT_F16;
+  p.wc.status = device_status_word();
+  p.wc.timeout = wait_timeout_ns();
+  if (p.wc.status == nullptr) return fail(H3B_ECUDA, "%s: device status word", what);
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= MAX_DEVICES) return fail(H3B_EUNSUPPORTED, "%s: device ordinal %d", what, dev);
+
+  CUtensorMap tmA, tmW;
+  int rc = weight_map(&tmW, o.w, o.K, o.N, o.E, o.ldw, o.E > 1 ? o.w_exp : o.ldw * ((o.N + 15) / 16 * 16));
+  if (rc) return rc;
+  // groups that can hold a row, and the row tiles that they can need at most
+  const int64_t active = o.T < o.E ? o.T : o.E;
+  const int64_t mean = (o.T + o.E - 1) / o.E;
+  if (mean > 128) {
+    p.num_nb = static_cast<int>((o.N + wide::BN - 1) / wide::BN);
+    const int64_t tiles = (o.T + active * (2 * wide::BM - 1)) / (2 * wide::BM) * p.num_nb;
+    if (tiles > most) return fail(H3B_EUNSUPPORTED, "%s: 2^31 tiles or more", what);
+    rc = load_map(&tmA, o.a, o.K, o.T, o.lda, wide::BM);
+    if (rc) return rc;
+    return launch_wide(p, tmA, tmW, tiles, dev, st);
+  }
+  const int nt = mean <= 16 ? 16 : (mean <= 32 ? 32 : (mean <= 64 ? 64 : 128));
+  p.num_nb = static_cast<int>((o.N + BLK - 1) / BLK);
+  const int64_t token_tiles = (o.T + active * (nt - 1)) / nt;
+  if (token_tiles > 65535) return fail(H3B_EUNSUPPORTED, "%s: %lld row tiles", what, (long long)token_tiles);
+  int split = 1;
+  while (split < narrow::MAX_SPLIT && token_tiles * p.num_nb * split < 2 * num_sms() && p.num_kb >= 8 * split) split *= 2;
+  if (static_cast<int64_t>(p.num_nb) * split > most) return fail(H3B_EUNSUPPORTED, "%s: 2^31 tiles or more", what);
+  rc = load_map(&tmA, o.a, o.K, o.T, o.lda, static_cast<uint32_t>(nt));
+  if (rc) return rc;
+  switch (nt) {
+    case 16: return launch_narrow<16>(p, tmA, tmW, token_tiles, split, dev, st);
+    case 32: return launch_narrow<32>(p, tmA, tmW, token_tiles, split, dev, st);
+    case 64: return launch_narrow<64>(p, tmA, tmW, token_tiles, split, dev, st);
+    default: return launch_narrow<128>(p, tmA, tmW, token_tiles, split, dev, st);
+  }
+}
+
+}  // namespace
+}  // namespace h3b
+
+using namespace h3b;
+
+extern "C" int h3b_fp8_gemm_blocks(const void* a, int64_t lda, const void* w, int64_t ldw, const float* sa, int64_t sa_row,
+                                   int64_t sa_block, const float* sb, int64_t sb_row, int64_t sb_block, const void* bias,
+                                   void* y, int64_t ldy, int64_t M, int64_t N, int64_t K, int32_t out_dtype,
+                                   h3b_stream_t stream) {
+  const Operands o{a, lda, w, ldw, 0, sa, sa_row, sa_block, sb, 0, sb_row, sb_block, bias, nullptr, 0, y, ldy, M, N, K, 1,
+                   out_dtype};
+  return gemm_blocks("fp8_gemm_blocks", o, reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" int h3b_fp8_gemm_grouped(const void* a, int64_t lda, const void* w, int64_t w_expert, int64_t ldw,
+                                    const float* sa, int64_t sa_row, int64_t sa_block, const float* sb, int64_t sb_expert,
+                                    int64_t sb_row, int64_t sb_block, const void* offsets, int32_t offsets_i64, void* y,
+                                    int64_t ldy, int64_t rows, int64_t experts, int64_t N, int64_t K, int32_t out_dtype,
+                                    h3b_stream_t stream) {
+  if (rows > 0 && offsets == nullptr) return fail(H3B_EINVAL, "fp8_gemm_grouped: offsets are required");
+  const Operands o{a,  lda, w, ldw, w_expert, sa,   sa_row, sa_block, sb,        sb_expert, sb_row, sb_block, nullptr, offsets,
+                   offsets_i64 != 0, y, ldy, rows, N, K, experts, out_dtype};
+  return gemm_blocks("fp8_gemm_grouped", o, reinterpret_cast<cudaStream_t>(stream));
+}

@@ -51,6 +51,13 @@ SIGNATURES = {
     "h3b_scale_swiglu_quant": (ctypes.c_int, [_p, _p, _p, _p, _p, _p, _i64, _i64, _i32, _p]),
     "h3b_fp8_gemm": (ctypes.c_int, [_p, _i64, _p, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i32, _i32,
                                     ctypes.POINTER(QkvSend), _p]),
+    "h3b_quant_blocks_e4m3": (ctypes.c_int, [_p, _i64, _i64, _i64, _p, _p, _i64, _i64, _i32, _p]),
+    "h3b_silu_mul_quant_blocks_e4m3": (ctypes.c_int, [_p, _i64, _i64, _i64, _p, _p, _i64, _i64, _i32, _p]),
+    "h3b_quant_weight_blocks_e4m3": (ctypes.c_int, [_p, _i64, _i64, _i64, _i64, _i64, _p, _p, _i32, _p]),
+    "h3b_fp8_gemm_blocks": (ctypes.c_int, [_p, _i64, _p, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _i64, _i64, _i64,
+                                           _i64, _i32, _p]),
+    "h3b_fp8_gemm_grouped": (ctypes.c_int, [_p, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _i64, _p, _i32,
+                                            _p, _i64, _i64, _i64, _i64, _i64, _i32, _p]),
     "h3b_flash_attn_fwd": (ctypes.c_int, [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _i64, _i64,
                                           _i64, _i32, _i32, _f32, _i32, _p, _p]),
     "h3b_flash_attn_fwd_bf16v": (ctypes.c_int, [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _i64,

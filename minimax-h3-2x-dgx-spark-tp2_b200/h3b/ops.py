@@ -454,6 +454,165 @@ def fp8_gemm_qkv_send(a: torch.Tensor, w: torch.Tensor, sa: torch.Tensor, sb: to
 
 
 # ---------------------------------------------------------------------------------------------------------------
+# block-scaled FP8: a scale per 128 values of a row (activations) or per 128 x 128 tile (weights)
+# ---------------------------------------------------------------------------------------------------------------
+
+BLOCK = 128
+
+
+def _nblocks(n: int) -> int:
+    return -(-n // BLOCK)
+
+
+def _launch(ref: torch.Tensor, name: str, *args) -> None:
+    """Call ``name`` with ``ref``'s device current, on that device's current torch stream."""
+    dev = ref.device.index
+    if dev is None or dev == torch.cuda.current_device():
+        _lib.call(name, *args, _stream(ref))
+        return
+    with torch.cuda.device(dev):
+        _lib.call(name, *args, _stream(ref))
+
+
+def _one_device(ref: torch.Tensor, what: str, *ts: torch.Tensor | None) -> None:
+    _need_cuda(ref, *ts)
+    for t in ts:
+        if t is not None and t.device != ref.device:
+            raise ValueError(f"{what}: tensors on {ref.device} and {t.device}")
+
+
+def _unit_rows(t: torch.Tensor, dtype: torch.dtype, dims: int, what: str) -> None:
+    """A ``dims``-dimensional tensor of ``dtype`` whose rows are dense (unit innermost stride)."""
+    if t.dtype != dtype:
+        raise TypeError(f"{what}: dtype {t.dtype}, expected {dtype}")
+    if t.dim() != dims or (t.stride(-1) != 1 and t.shape[-1] > 1):
+        raise ValueError(f"{what}: must have {dims} dimensions and unit innermost stride, got {tuple(t.shape)} with "
+                         f"strides {t.stride()}")
+
+
+def _row_scales(rows: int, cols: int, like: torch.Tensor) -> torch.Tensor:
+    """Scales [rows, ceil(cols / 128)] stored block by block (strides (1, rows rounded up to 4)): a tile's row scales of
+    one block are then consecutive in memory, which is how the products read them."""
+    return torch.empty_strided((rows, _nblocks(cols)), (1, max(rows + 3 & ~3, 4)), dtype=torch.float32,
+                               device=like.device)
+
+
+def quant_blocks(h: torch.Tensor, *, div_mode: int = DIV_IEEE) -> tuple[torch.Tensor, torch.Tensor]:
+    """Block quant of bf16 rows h [M, K] (unit column stride, any row stride): (q [M, K] e4m3, scale [M, ceil(K/128)]
+    fp32), the per-token quant's scale and rounding taken over each 128 columns.  The scale tensor is stored block by
+    block (unit stride along M)."""
+    _need_cuda(h)
+    _unit_rows(h, torch.bfloat16, 2, "quant_blocks h")
+    m, k = h.shape
+    q = torch.empty((m, k), dtype=E4M3, device=h.device)
+    s = _row_scales(m, k, h)
+    _launch(h, "h3b_quant_blocks_e4m3", h.data_ptr(), m, k, h.stride(0), q.data_ptr(), s.data_ptr(), s.stride(0),
+            s.stride(1), div_mode)
+    return q, s
+
+
+def silu_mul_quant_blocks(x: torch.Tensor, *, div_mode: int = DIV_IEEE) -> tuple[torch.Tensor, torch.Tensor]:
+    """silu(gate) * up of bf16 x [M, 2F] (gate columns, then up columns), in fp32, then the block quant: (q [M, F] e4m3,
+    scale [M, ceil(F/128)] fp32).  The product is not rounded to bf16 in between (``silu_mul_quant`` does)."""
+    _need_cuda(x)
+    _unit_rows(x, torch.bfloat16, 2, "silu_mul_quant_blocks x")
+    m, width = x.shape
+    if width % 2:
+        raise ValueError(f"silu_mul_quant_blocks: x must be [rows, 2F], got {tuple(x.shape)}")
+    q = torch.empty((m, width // 2), dtype=E4M3, device=x.device)
+    s = _row_scales(m, width // 2, x)
+    _launch(x, "h3b_silu_mul_quant_blocks_e4m3", x.data_ptr(), m, width // 2, x.stride(0), q.data_ptr(), s.data_ptr(),
+            s.stride(0), s.stride(1), div_mode)
+    return q, s
+
+
+def quant_weight_blocks(w: torch.Tensor, *, div_mode: int = DIV_IEEE) -> tuple[torch.Tensor, torch.Tensor]:
+    """Tile quant of a bf16 weight [N, K], or of one per expert [E, N, K]: e4m3 of the same shape and an fp32 scale per
+    128 x 128 tile, [N / 128, K / 128] (or [E, N / 128, K / 128]), rounded up."""
+    _need_cuda(w)
+    if w.dim() not in (2, 3):
+        raise ValueError(f"quant_weight_blocks: w must be [N, K] or [E, N, K], got {tuple(w.shape)}")
+    _unit_rows(w, torch.bfloat16, w.dim(), "quant_weight_blocks w")
+    n, k = w.shape[-2:]
+    e = w.shape[0] if w.dim() == 3 else 1
+    q = torch.empty(w.shape, dtype=E4M3, device=w.device)
+    s = torch.empty((*w.shape[:-2], _nblocks(n), _nblocks(k)), dtype=torch.float32, device=w.device)
+    _launch(w, "h3b_quant_weight_blocks_e4m3", w.data_ptr(), e, n, k, w.stride(0) if w.dim() == 3 else 0, w.stride(-2),
+            q.data_ptr(), s.data_ptr(), div_mode)
+    return q, s
+
+
+def _block_product(a, w, sa, sb, bias, out_dtype, out, what: str, offsets=None):  # noqa: ANN001,ANN202
+    """The arguments that both block-scaled products share, checked; returns the output tensor."""
+    _one_device(a, what, w, sa, sb, bias, offsets, out)
+    _unit_rows(a, E4M3, 2, f"{what} a")
+    _unit_rows(w, E4M3, 2 if offsets is None else 3, f"{what} w")
+    m, k = a.shape
+    n = w.shape[-2]
+    if w.shape[-1] != k or k < 16 or k % 16 or n < 1:
+        raise ValueError(f"{what}: a {tuple(a.shape)} and w {tuple(w.shape)} need the same K, a multiple of 16")
+    if sa.dtype != torch.float32 or sb.dtype != torch.float32:
+        raise TypeError(f"{what}: scales must be fp32, got {sa.dtype} and {sb.dtype}")
+    kb = _nblocks(k)
+    if tuple(sa.shape) != (m, kb) or tuple(sb.shape) != (*w.shape[:-2], _nblocks(n), kb):
+        raise ValueError(f"{what}: sa must be {(m, kb)} and sb {(*w.shape[:-2], _nblocks(n), kb)}, got "
+                         f"{tuple(sa.shape)} and {tuple(sb.shape)}")
+    if out is None:
+        if out_dtype not in (torch.bfloat16, torch.float16):
+            raise TypeError(f"{what}: out_dtype {out_dtype}, expected bf16 or f16")
+        return torch.empty((m, n), dtype=out_dtype, device=a.device)
+    _dt(out, torch.bfloat16, torch.float16, what=f"{what} out")
+    if tuple(out.shape) != (m, n) or (n > 1 and out.stride(1) != 1) or (m > 1 and out.stride(0) < n):
+        raise ValueError(f"{what}: out must be [{m}, {n}] with unit column stride and rows that do not overlap, got "
+                         f"{tuple(out.shape)} with strides {out.stride()}")
+    return out
+
+
+def _ld(t: torch.Tensor) -> int:
+    """The row stride of a matrix; a single row may have any, and K (a multiple of 16) serves."""
+    return t.stride(-2) if t.shape[-2] > 1 else t.shape[-1]
+
+
+def fp8_gemm_blocks(a: torch.Tensor, w: torch.Tensor, sa: torch.Tensor, sb: torch.Tensor,
+                    bias: torch.Tensor | None = None, out_dtype: torch.dtype = torch.bfloat16,
+                    out: torch.Tensor | None = None) -> torch.Tensor:
+    """y [M, N] of block-scaled operands: a [M, K] e4m3 with sa [M, ceil(K/128)] fp32 (``quant_blocks``), w [N, K] e4m3
+    with sb [ceil(N/128), ceil(K/128)] fp32 (``quant_weight_blocks`` or a block-quantised checkpoint); scales of any
+    strides.  K a multiple of 16, row strides of a and w too; any M and N.  fp32 sums, one rounding to out_dtype (bf16
+    or f16); ``bias`` [N] bf16 is added before it."""
+    y = _block_product(a, w, sa, sb, bias, out_dtype, out, "fp8_gemm_blocks")
+    m, k = a.shape
+    n = w.shape[0]
+    bias = _bias(bias, n, "fp8_gemm_blocks")
+    _launch(a, "h3b_fp8_gemm_blocks", a.data_ptr(), _ld(a), w.data_ptr(), _ld(w), sa.data_ptr(), sa.stride(0),
+            sa.stride(1), sb.data_ptr(), sb.stride(0), sb.stride(1), _ptr(bias), y.data_ptr(), max(y.stride(0), n), m, n,
+            k, OUT_BF16 if y.dtype == torch.bfloat16 else OUT_F16)
+    return y
+
+
+def fp8_gemm_grouped(a: torch.Tensor, w: torch.Tensor, sa: torch.Tensor, sb: torch.Tensor, offsets: torch.Tensor,
+                     out_dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``fp8_gemm_blocks`` with one weight per expert: rows offsets[e] .. offsets[e+1] of a [T, K] (sorted by expert)
+    times w[e] of w [E, N, K], with sb [E, ceil(N/128), ceil(K/128)].  ``offsets``: E + 1 int32 or int64 values on the
+    device, non-decreasing within [0, T]; the host never reads them.  Groups may be empty.  Rows before offsets[0] and
+    from offsets[E] on are not written (a fresh output is uninitialised there).  Bounds out of order or out of range
+    skip their group and record H3B_EINVAL in the device status word (``device_status``)."""
+    if offsets.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"fp8_gemm_grouped: offsets {offsets.dtype}, expected int32 or int64")
+    y = _block_product(a, w, sa, sb, None, out_dtype, out, "fp8_gemm_grouped", offsets)
+    m, k = a.shape
+    e, n = w.shape[:2]
+    if tuple(offsets.shape) != (e + 1,) or e < 1:
+        raise ValueError(f"fp8_gemm_grouped: offsets must be [{e + 1}] for {e} experts, got {tuple(offsets.shape)}")
+    offsets = offsets.contiguous()
+    _launch(a, "h3b_fp8_gemm_grouped", a.data_ptr(), _ld(a), w.data_ptr(), w.stride(0), _ld(w), sa.data_ptr(),
+            sa.stride(0), sa.stride(1), sb.data_ptr(), sb.stride(0), sb.stride(1), sb.stride(2), offsets.data_ptr(),
+            int(offsets.dtype == torch.int64), y.data_ptr(), max(y.stride(0), n), m, e, n, k,
+            OUT_BF16 if y.dtype == torch.bfloat16 else OUT_F16)
+    return y
+
+
+# ---------------------------------------------------------------------------------------------------------------
 # attention
 # ---------------------------------------------------------------------------------------------------------------
 
@@ -686,6 +845,17 @@ SCHEMAS = {
                      "Tensor? bias) -> Tensor",
     "fp8_gemm_gate_out": "fp8_gemm_gate_out(Tensor a, Tensor w, Tensor sa, Tensor sb, Tensor x, Tensor gate, "
                          "Tensor indices, Tensor? bias, Tensor(a!) out) -> ()",
+    "quant_blocks": "quant_blocks(Tensor h, int div_mode=0) -> (Tensor, Tensor)",
+    "quant_weight_blocks": "quant_weight_blocks(Tensor w, int div_mode=0) -> (Tensor, Tensor)",
+    "silu_mul_quant_blocks": "silu_mul_quant_blocks(Tensor x, int div_mode=0) -> (Tensor, Tensor)",
+    "fp8_gemm_blocks": "fp8_gemm_blocks(Tensor a, Tensor w, Tensor sa, Tensor sb, Tensor? bias, ScalarType out_dtype) "
+                       "-> Tensor",
+    "fp8_gemm_blocks_out": "fp8_gemm_blocks_out(Tensor a, Tensor w, Tensor sa, Tensor sb, Tensor? bias, "
+                           "Tensor(a!) out) -> ()",
+    "fp8_gemm_grouped": "fp8_gemm_grouped(Tensor a, Tensor w, Tensor sa, Tensor sb, Tensor offsets, "
+                        "ScalarType out_dtype) -> Tensor",
+    "fp8_gemm_grouped_out": "fp8_gemm_grouped_out(Tensor a, Tensor w, Tensor sa, Tensor sb, Tensor offsets, "
+                            "Tensor(a!) out) -> ()",
     "flash_attn": "flash_attn(Tensor q, Tensor k, Tensor v, float? scale=None, int? valid_kv=None) -> Tensor",
     "flash_attn_scratch": "flash_attn_scratch(Tensor q, Tensor k, Tensor v, float? scale, int? valid_kv, "
                           "Tensor(a!) v16, Tensor(b!) ctl) -> Tensor",
@@ -709,6 +879,15 @@ def _kernels() -> dict:
         "fp8_gemm_gate": lambda a, w, sa, sb, x, g, idx, bias: fp8_gemm_gate(a, w, sa, sb, x, g, idx, bias),
         "fp8_gemm_gate_out": lambda a, w, sa, sb, x, g, idx, bias, out: (
             fp8_gemm_gate(a, w, sa, sb, x, g, idx, bias, out=out), None)[1],
+        "quant_blocks": lambda h, div_mode=DIV_IEEE: quant_blocks(h, div_mode=div_mode),
+        "quant_weight_blocks": lambda w, div_mode=DIV_IEEE: quant_weight_blocks(w, div_mode=div_mode),
+        "silu_mul_quant_blocks": lambda x, div_mode=DIV_IEEE: silu_mul_quant_blocks(x, div_mode=div_mode),
+        "fp8_gemm_blocks": lambda a, w, sa, sb, bias, dt: fp8_gemm_blocks(a, w, sa, sb, bias, dt),
+        "fp8_gemm_blocks_out": lambda a, w, sa, sb, bias, out: (
+            fp8_gemm_blocks(a, w, sa, sb, bias, out=out), None)[1],
+        "fp8_gemm_grouped": lambda a, w, sa, sb, off, dt: fp8_gemm_grouped(a, w, sa, sb, off, dt),
+        "fp8_gemm_grouped_out": lambda a, w, sa, sb, off, out: (
+            fp8_gemm_grouped(a, w, sa, sb, off, out=out), None)[1],
         "flash_attn": lambda q, k, v, scale=None, valid_kv=None: flash_attn(q, k, v, scale=scale, valid_kv=valid_kv),
         "flash_attn_scratch": lambda q, k, v, scale, valid_kv, v16, ctl: flash_attn(q, k, v, scale=scale,
                                                                                     valid_kv=valid_kv, v16=v16,
@@ -721,6 +900,10 @@ def _fakes() -> dict:
 
     def q_and_s(rows, cols, like):
         return like.new_empty((rows, cols), dtype=E4M3), like.new_empty((rows, 1), dtype=f32)
+
+    def q_and_block_s(rows, cols, like):
+        s = like.new_empty_strided((rows, _nblocks(cols)), (1, max(rows + 3 & ~3, 4)), dtype=f32)
+        return like.new_empty((rows, cols), dtype=E4M3), s
 
     def attn_out(q):
         return q.new_empty(q.shape, dtype=torch.bfloat16)
@@ -741,6 +924,15 @@ def _fakes() -> dict:
         "fp8_gemm_gate": lambda a, w, sa, sb, x, g, idx, bias: x.new_empty((a.shape[0], w.shape[0]),
                                                                            dtype=torch.bfloat16),
         "fp8_gemm_gate_out": lambda a, w, sa, sb, x, g, idx, bias, out: None,
+        "quant_blocks": lambda h, div_mode=0: q_and_block_s(h.shape[0], h.shape[1], h),
+        "quant_weight_blocks": lambda w, div_mode=0: (
+            w.new_empty(w.shape, dtype=E4M3),
+            w.new_empty((*w.shape[:-2], _nblocks(w.shape[-2]), _nblocks(w.shape[-1])), dtype=f32)),
+        "silu_mul_quant_blocks": lambda x, div_mode=0: q_and_block_s(x.shape[0], x.shape[1] // 2, x),
+        "fp8_gemm_blocks": lambda a, w, sa, sb, bias, dt: a.new_empty((a.shape[0], w.shape[0]), dtype=dt),
+        "fp8_gemm_blocks_out": lambda a, w, sa, sb, bias, out: None,
+        "fp8_gemm_grouped": lambda a, w, sa, sb, off, dt: a.new_empty((a.shape[0], w.shape[1]), dtype=dt),
+        "fp8_gemm_grouped_out": lambda a, w, sa, sb, off, out: None,
         "flash_attn": lambda q, k, v, scale=None, valid_kv=None: attn_out(q),
         "flash_attn_scratch": lambda q, k, v, scale, valid_kv, v16, ctl: attn_out(q),
     }
