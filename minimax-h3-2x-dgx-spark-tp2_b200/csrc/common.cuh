@@ -82,7 +82,7 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
 
 // Bounded wait for the phase of `parity` to complete.  Returns false (and records H3B_ETIMEOUT once) when the bound
 // expires, or when another thread of the grid already recorded a failure.
-static __device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, WaitCtl w) {
+__device__ __forceinline__ bool mbar_wait_loop(uint32_t bar, uint32_t parity, const WaitCtl& w) {
   const uint64_t t0 = globaltimer();
   while (true) {
 #pragma unroll 1
@@ -95,9 +95,17 @@ static __device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity
     }
   }
 }
+static __device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, WaitCtl w) {
+  return mbar_wait_loop(bar, parity, w);
+}
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const WaitCtl& w) {
   if (mbar_try_wait(bar, parity)) return true;
   return mbar_wait_slow(bar, parity, w);
+}
+// the same without a call: for code after setmaxnreg, where a call would hold ptxas to the launch's register count
+__device__ __forceinline__ bool mbar_wait_inline(uint32_t bar, uint32_t parity, const WaitCtl& w) {
+  if (mbar_try_wait(bar, parity)) return true;
+  return mbar_wait_loop(bar, parity, w);
 }
 
 // ---- TMA (no multicast anywhere in this library) ----

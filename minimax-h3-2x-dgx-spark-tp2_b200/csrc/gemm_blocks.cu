@@ -69,7 +69,7 @@ struct Walk {
   int e;               // the tile found: expert, its rows [lo, hi), row blocks and the tile's index within the expert
   int64_t lo, hi;
   int blocks, r;
-  __device__ bool find(const Params& p, int64_t t, int per_block) {
+  __device__ __forceinline__ bool find(const Params& p, int64_t t, int per_block) {
     const int lane = threadIdx.x & 31;
     while (e0 < p.experts) {
       int64_t l = 0, h = 0;
@@ -125,7 +125,7 @@ namespace wide {
 
 constexpr int BM = 128, BN = 256, STAGES = 6;
 constexpr int STAGE_BYTES = 2 * BM * BLK;           // this CTA's 128 rows of a and 128 rows of w, 128 bytes each
-constexpr int EPI_WARPS = 8, THREADS = 64 + 32 * EPI_WARPS;
+constexpr int EPI_WARPS = 8, FIRST_EPI = 4, THREADS = 32 * (FIRST_EPI + EPI_WARPS);
 constexpr int WARP_STAGING = 32 * 128;              // 32 rows x 64 columns of 16-bit output
 constexpr int SMEM = STAGES * STAGE_BYTES + 1024 + 1024 + EPI_WARPS * WARP_STAGING;
 static_assert(SMEM <= 232448, "shared memory");
@@ -149,29 +149,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE_BYTES);
-  // bars: full[STAGES], empty[STAGES], tfull[2], tempty[2], done; then the TMEM address and the start flag
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 5);
+  // bars: full[STAGES], used[STAGES], tempty[2], done; then the TMEM address and the start flag.  used[s]: the MMAs of
+  // the step in stage s are complete, which frees the stage for the producer and hands the step's accumulator to the
+  // epilogue (one commit per step for both)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 3);
   uint32_t* start_flag = tmem_slot + 1;
   uint8_t* staging = smem + STAGES * STAGE_BYTES + 1024;
   const uint32_t smem0 = smem_u32(smem), bar0 = smem_u32(bars);
   auto full_bar = [&](int s) { return bar0 + 8u * s; };
-  auto empty_bar = [&](int s) { return bar0 + 8u * (STAGES + s); };
-  auto tfull_bar = [&](int b) { return bar0 + 8u * (2 * STAGES + b); };
-  auto tempty_bar = [&](int b) { return bar0 + 8u * (2 * STAGES + 2 + b); };
-  const uint32_t done_bar = bar0 + 8u * (2 * STAGES + 4);
+  auto used_bar = [&](int s) { return bar0 + 8u * (STAGES + s); };
+  auto tempty_bar = [&](int b) { return bar0 + 8u * (2 * STAGES + b); };
+  const uint32_t done_bar = bar0 + 8u * (2 * STAGES + 2);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int crank = static_cast<int>(cluster_ctarank());  // 0: the pair's leader (issues the MMAs)
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(full_bar(s), 1);
-      mbar_init(empty_bar(s), 1);
+      mbar_init(used_bar(s), 1);
     }
-    for (int b = 0; b < 2; ++b) {
-      mbar_init(tfull_bar(b), 1);
-      mbar_init(tempty_bar(b), 2 * EPI_WARPS);  // one arrival per epilogue warp of both CTAs, on the leader's
-    }
-    mbar_init(done_bar, 1);
+    for (int b = 0; b < 2; ++b) mbar_init(tempty_bar(b), 2 * EPI_WARPS);  // every epilogue warp of both CTAs
+    mbar_init(done_bar, 2);
     fence_mbar_init();
     *start_flag = status_bad(p.wc) ? 0u : 1u;
     tma_prefetch_desc(&tmA);
@@ -189,13 +187,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   const int first_tile = static_cast<int>(cluster_id_x()), tile_step = static_cast<int>(cluster_count_x());
   Walk<2 * BM> walk;
 
-  if (start) {
-    if (warp == 0) {
+  if (warp < FIRST_EPI) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (start && warp == 0) {
       // ---------------- TMA producer (both CTAs; stages complete on the leader's full barrier) ----------------
       const uint32_t lead_full0 = mapa_shared(full_bar(0), 0);
       int stage = 0;
       uint32_t phase = 0;
-      uint32_t used = 0, last = 0;  // per stage: loaded at all, parity of its last load
+      uint32_t loaded = 0, last = 0;  // per stage: loaded at all, parity of its last load
       bool ok = true;
       for (int64_t t = first_tile; ok && walk.find(p, t, p.num_nb); t += tile_step) {
         int mb, nb;
@@ -204,7 +203,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         const int wrow = nb * BN + crank * BM;
         if (lane == 0) {
           for (int kb = 0; kb < p.num_kb; ++kb) {
-            if (!mbar_wait(empty_bar(stage), phase ^ 1u, p.wc)) {
+            if (!mbar_wait_inline(used_bar(stage), phase ^ 1u, p.wc)) {
               ok = false;
               break;
             }
@@ -212,7 +211,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             if (crank == 0) mbar_arrive_expect_tx(full_bar(stage), 2 * STAGE_BYTES);
             tma_load_2d_pair(sA, &tmA, lead_full0 + 8u * stage, kb * BLK, arow);
             tma_load_3d_pair(sA + BM * BLK, &tmW, lead_full0 + 8u * stage, kb * BLK, wrow, walk.e);
-            used |= 1u << stage;
+            loaded |= 1u << stage;
             last = (last & ~(1u << stage)) | (phase << stage);
             if (++stage == STAGES) {
               stage = 0;
@@ -227,25 +226,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       // consumed it.
       if (lane == 0) {
         for (int s = 0; s < STAGES; ++s) {
-          if (!(used >> s & 1u)) continue;
-          const uint32_t bar = crank == 0 ? full_bar(s) : empty_bar(s), par = last >> s & 1u;
+          if (!(loaded >> s & 1u)) continue;
+          const uint32_t bar = crank == 0 ? full_bar(s) : used_bar(s), par = last >> s & 1u;
           const uint64_t t0 = globaltimer();
           while (!mbar_try_wait(bar, par) && globaltimer() - t0 < p.wc.timeout) {
           }
         }
       }
-    } else if (warp == 1) {
+    } else if (start && (warp == 1 || warp == 2)) {
       if (crank == 0) {
-        // ---------------- MMA issuer (the leader only): one accumulator per 128-value step of K ----------------
-        int stage = 0;
-        uint32_t phase = 0;
-        uint32_t it = 0;  // steps so far: TMEM buffer it & 1
+        // ---------------- MMA issuers (the leader only): one accumulator per 128-value step of K ----------------
+        // Two warps take the steps in turn, each with a TMEM buffer of its own: a thread that issues MMAs is held while
+        // the tensor pipe is busy, and its waits and commits (~350 cycles a step) would leave the pipe idle.
+        const int b = warp - 1;
+        uint32_t it = 0;  // steps before this tile
         bool ok = true;
-        for (int64_t t = first_tile; ok && walk.find(p, t, p.num_nb); t += tile_step) {
+        for (int64_t t = first_tile; ok && walk.find(p, t, p.num_nb); t += tile_step, it += p.num_kb) {
           if (lane == 0) {
-            for (int kb = 0; kb < p.num_kb; ++kb, ++it) {
-              const int b = it & 1;
-              if (!mbar_wait(tempty_bar(b), ((it >> 1) & 1u) ^ 1u, p.wc) || !mbar_wait(full_bar(stage), phase, p.wc)) {
+            for (uint32_t i = it + ((it ^ b) & 1u); i < it + p.num_kb; i += 2) {
+              const uint32_t round = i / STAGES, stage = i - round * STAGES;
+              if (!mbar_wait_inline(full_bar(stage), round & 1u, p.wc) ||
+                  !mbar_wait_inline(tempty_bar(b), ((i >> 1) & 1u) ^ 1u, p.wc)) {
                 ok = false;
                 break;
               }
@@ -255,12 +256,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 #pragma unroll
               for (int kk = 0; kk < BLK / 32; ++kk)
                 umma_f8_ss_pair(tmem_base + static_cast<uint32_t>(b * BN), adesc + 2u * kk, bdesc + 2u * kk, IDESC, kk != 0);
-              umma_commit_pair_mc(tfull_bar(b), 3);
-              umma_commit_pair_mc(empty_bar(stage), 3);
-              if (++stage == STAGES) {
-                stage = 0;
-                phase ^= 1u;
-              }
+              umma_commit_pair_mc(used_bar(stage), 3);
             }
           }
           ok = __shfl_sync(0xffffffffu, ok, 0);
@@ -272,13 +268,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           }
         }
       }
-    } else {
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+    if (start) {
       // ---------------- epilogue warps: 32 rows x 128 columns of running sums each ----------------
-      const int sub = warp & 3, half = (warp - 2) >> 2;
+      const int sub = warp & 3, half = (warp - FIRST_EPI) >> 2;
       const uint32_t tmine = tmem_base + (static_cast<uint32_t>(sub * 32) << 16) + static_cast<uint32_t>(half * 128);
       const uint32_t lead_tempty0 = mapa_shared(tempty_bar(0), 0);
-      uint4* stg = reinterpret_cast<uint4*>(staging + (warp - 2) * WARP_STAGING);
-      uint32_t it = 0;
+      uint4* stg = reinterpret_cast<uint4*>(staging + (warp - FIRST_EPI) * WARP_STAGING);
+      uint32_t it = 0, phase = 0;
+      int stage = 0;
       bool ok = true;
       for (int64_t t = first_tile; ok && walk.find(p, t, p.num_nb); t += tile_step) {
         int mb, nb;
@@ -304,26 +304,39 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             sb1 = __ldg(sbp + (kb + 2) * p.sb_blk);
           }
           const int b = it & 1;
-          if (!__all_sync(0xffffffffu, mbar_wait(tfull_bar(b), (it >> 1) & 1u, p.wc))) {
+          if (!__all_sync(0xffffffffu, mbar_wait_inline(used_bar(stage), phase, p.wc))) {
             ok = false;  // for the whole warp: the TMEM loads below need all of it
             break;
           }
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
           tc_fence_after();
           const uint32_t tcur = tmine + static_cast<uint32_t>(b * BN);
+          // 32-column slices, two ahead: the buffer is read (and given back) after half of the additions
+          uint32_t ra[32], rb[32];
+          auto add = [&](const uint32_t (&r)[32], int c) {
 #pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            uint32_t r[16];
-            tmem_ld16(tcur + 16 * c, r);
-            tmem_ld_wait();
-            reg_fence(r);
-            if (c == 7) {  // this warp has read the buffer: the next step's MMAs may overwrite it
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive_cluster_relaxed(lead_tempty0 + 8u * b);
-            }
-#pragma unroll
-            for (int i = 0; i < 16; ++i) acc[16 * c + i] = fmaf(__uint_as_float(r[i]), s, acc[16 * c + i]);
-          }
+            for (int i = 0; i < 32; ++i) acc[c + i] = fmaf(__uint_as_float(r[i]), s, acc[c + i]);
+          };
+          tmem_ld32(tcur, ra);
+          tmem_ld32(tcur + 32, rb);
+          tmem_ld_wait();
+          reg_fence(ra);
+          reg_fence(rb);
+          add(ra, 0);
+          tmem_ld32(tcur + 64, ra);
+          add(rb, 32);
+          tmem_ld32(tcur + 96, rb);
+          tmem_ld_wait();
+          reg_fence(ra);
+          reg_fence(rb);
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster_relaxed(lead_tempty0 + 8u * b);
+          add(ra, 64);
+          add(rb, 96);
         }
         if (!ok) break;
         if (p.bias != nullptr) {
