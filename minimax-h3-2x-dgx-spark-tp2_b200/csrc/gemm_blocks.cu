@@ -7,10 +7,10 @@
 // K step of 128 is its own accumulator in TMEM, and the epilogue warps add it, scaled, to fp32 running sums in
 // registers while the next step's MMAs fill the other TMEM buffer.  Both forms below are that loop:
 //
-//   wide    (many rows): CTA pairs with 2-SM MMAs over 256 rows x 256 columns.  Thread = output row, so sa * sb is one
+//   wide    (over 64 rows a group): CTA pairs with 2-SM MMAs over 256 rows x 256 columns.  Thread = output row, so sa * sb is one
 //           scalar per thread and step and the promotion costs one FMA per element: 8 warps x 128 FMAs per 512 tensor
 //           cycles.  128 running sums per thread, two 256-column TMEM buffers.
-//   narrow  (few rows): the operands swapped, D^T = w a^T: 128 weight rows x NT tokens (NT = 16 .. 128) per CTA, so that
+//   narrow  (few rows): the operands swapped, D^T = w a^T: 128 weight rows x NT tokens (NT = 16, 32 or 64) per CTA, so that
 //           a tile streams the weight once with no tensor work on absent rows.  K is split over a cluster of CTAs that
 //           add their sums through distributed shared memory in a fixed order (the result does not depend on timing).
 //
@@ -29,6 +29,7 @@ struct Params {
   int64_t T, N;       // rows of a, rows of w (of one expert)
   int num_kb;         // 128-value blocks of K
   int num_nb;         // column tiles (256 wide, or 128 weight rows narrow)
+  int split;          // CTAs (wide: pairs of CTAs) of a cluster that share a tile, each with a part of K
   int experts;        // groups; dense: 1 without offsets
   const void* offsets;
   int off64;          // offsets are int64 (else int32)
@@ -126,6 +127,7 @@ namespace wide {
 constexpr int BM = 128, BN = 256, STAGES = 6;
 constexpr int STAGE_BYTES = 2 * BM * BLK;           // this CTA's 128 rows of a and 128 rows of w, 128 bytes each
 constexpr int EPI_WARPS = 8, FIRST_EPI = 4, THREADS = 32 * (FIRST_EPI + EPI_WARPS);
+constexpr int MAX_SPLIT = 4, ROUND_COST = 14;        // a cluster of 8 CTAs at most
 constexpr int WARP_STAGING = 32 * 128;              // 32 rows x 64 columns of 16-bit output
 constexpr int SMEM = STAGES * STAGE_BYTES + 1024 + 1024 + EPI_WARPS * WARP_STAGING;
 static_assert(SMEM <= 232448, "shared memory");
@@ -143,7 +145,9 @@ __device__ __forceinline__ void coords(int r, int blocks, int num_nb, int& mb, i
   nb = q / size;
 }
 
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+// SPLIT: clusters of p.split pairs take a tile each, every pair a part of K
+template <bool SPLIT>
+__global__ void __launch_bounds__(THREADS, 1)
     kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
            const __grid_constant__ CUtensorMap tmY, const __grid_constant__ Params p) {
   extern __shared__ uint8_t smem_raw[];
@@ -162,7 +166,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   const uint32_t done_bar = bar0 + 8u * (2 * STAGES + 2);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int crank = static_cast<int>(cluster_ctarank());  // 0: the pair's leader (issues the MMAs)
+  const uint32_t rank = cluster_ctarank(), leader = SPLIT ? rank & ~1u : 0u;
+  const int crank = static_cast<int>(rank & 1u);  // 0: the pair's leader (issues the MMAs)
+  const int part = SPLIT ? static_cast<int>(rank >> 1) : 0;  // the pair's part of K: steps [kb0, kb1)
+  const int kb0 = SPLIT ? static_cast<int>(static_cast<int64_t>(p.num_kb) * part / p.split) : 0;
+  const int kb1 = SPLIT ? static_cast<int>(static_cast<int64_t>(p.num_kb) * (part + 1) / p.split) : p.num_kb;
+  const uint16_t pair_mask = static_cast<uint16_t>(3u << leader);
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(full_bar(s), 1);
@@ -183,7 +192,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   cluster_sync();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  const bool start = cluster_flag(smem_u32(start_flag));
+  const bool start = cluster_flag(smem_u32(start_flag));  // of the cluster's first CTA
   const int first_tile = static_cast<int>(cluster_id_x()), tile_step = static_cast<int>(cluster_count_x());
   Walk<2 * BM> walk;
 
@@ -191,7 +200,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     if (start && warp == 0) {
       // ---------------- TMA producer (both CTAs; stages complete on the leader's full barrier) ----------------
-      const uint32_t lead_full0 = mapa_shared(full_bar(0), 0);
+      const uint32_t lead_full0 = mapa_shared(full_bar(0), leader);
       int stage = 0;
       uint32_t phase = 0;
       uint32_t loaded = 0, last = 0;  // per stage: loaded at all, parity of its last load
@@ -202,7 +211,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         const int arow = static_cast<int>(walk.lo) + (2 * mb + crank) * BM;
         const int wrow = nb * BN + crank * BM;
         if (lane == 0) {
-          for (int kb = 0; kb < p.num_kb; ++kb) {
+          for (int kb = kb0; kb < kb1; ++kb) {
             if (!mbar_wait_inline(used_bar(stage), phase ^ 1u, p.wc)) {
               ok = false;
               break;
@@ -241,9 +250,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         const int b = warp - 1;
         uint32_t it = 0;  // steps before this tile
         bool ok = true;
-        for (int64_t t = first_tile; ok && walk.find(p, t, p.num_nb); t += tile_step, it += p.num_kb) {
+        for (int64_t t = first_tile; ok && walk.find(p, t, p.num_nb); t += tile_step, it += kb1 - kb0) {
           if (lane == 0) {
-            for (uint32_t i = it + ((it ^ b) & 1u); i < it + p.num_kb; i += 2) {
+            for (uint32_t i = it + ((it ^ b) & 1u); i < it + (kb1 - kb0); i += 2) {
               const uint32_t round = i / STAGES, stage = i - round * STAGES;
               if (!mbar_wait_inline(full_bar(stage), round & 1u, p.wc) ||
                   !mbar_wait_inline(tempty_bar(b), ((i >> 1) & 1u) ^ 1u, p.wc)) {
@@ -256,7 +265,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 #pragma unroll
               for (int kk = 0; kk < BLK / 32; ++kk)
                 umma_f8_ss_pair(tmem_base + static_cast<uint32_t>(b * BN), adesc + 2u * kk, bdesc + 2u * kk, IDESC, kk != 0);
-              umma_commit_pair_mc(used_bar(stage), 3);
+              umma_commit_pair_mc(used_bar(stage), pair_mask);
             }
           }
           ok = __shfl_sync(0xffffffffu, ok, 0);
@@ -269,37 +278,46 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         }
       }
     }
+    if constexpr (SPLIT) {  // the barriers of the epilogue's end phase
+      __syncwarp();
+      __syncthreads();
+      cluster_sync();
+    }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
     if (start) {
       // ---------------- epilogue warps: 32 rows x 128 columns of running sums each ----------------
       const int sub = warp & 3, half = (warp - FIRST_EPI) >> 2;
       const uint32_t tmine = tmem_base + (static_cast<uint32_t>(sub * 32) << 16) + static_cast<uint32_t>(half * 128);
-      const uint32_t lead_tempty0 = mapa_shared(tempty_bar(0), 0);
+      const uint32_t lead_tempty0 = mapa_shared(tempty_bar(0), leader);
       uint4* stg = reinterpret_cast<uint4*>(staging + (warp - FIRST_EPI) * WARP_STAGING);
       uint32_t it = 0, phase = 0;
       int stage = 0;
-      bool ok = true;
+      bool ok = true, have = false;
+      float acc[128];
+      int mb = 0, nb = 0;
       for (int64_t t = first_tile; ok && walk.find(p, t, p.num_nb); t += tile_step) {
-        int mb, nb;
         coords(walk.r, walk.blocks, p.num_nb, mb, nb);
         const int64_t m0 = walk.lo + (2 * mb + crank) * BM + sub * 32;  // the warp's first row
         const int64_t n0 = static_cast<int64_t>(nb) * BN + half * 128;  // and first column
         const bool row_ok = m0 + lane < walk.hi, col_ok = n0 < p.N;
         const float* sap = p.sa + (row_ok ? m0 + lane : walk.lo) * p.sa_row;
         const float* sbp = p.sb + walk.e * p.sb_exp + (col_ok ? n0 / BLK : 0) * p.sb_row;
-        float acc[128];
 #pragma unroll
         for (int i = 0; i < 128; ++i) acc[i] = 0.0f;
         // the scales of the next two steps are on their way while a step is added
-        float sa0 = __ldg(sap), sb0 = __ldg(sbp);
-        float sa1 = p.num_kb > 1 ? __ldg(sap + p.sa_blk) : 0.0f, sb1 = p.num_kb > 1 ? __ldg(sbp + p.sb_blk) : 0.0f;
+        float sa0 = __ldg(sap + kb0 * p.sa_blk), sb0 = __ldg(sbp + kb0 * p.sb_blk);
+        float sa1 = 0.0f, sb1 = 0.0f;
+        if (kb0 + 1 < kb1) {
+          sa1 = __ldg(sap + (kb0 + 1) * p.sa_blk);
+          sb1 = __ldg(sbp + (kb0 + 1) * p.sb_blk);
+        }
 #pragma unroll 1
-        for (int kb = 0; kb < p.num_kb; ++kb, ++it) {
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
           const float s = sa0 * sb0;
           sa0 = sa1;
           sb0 = sb1;
-          if (kb + 2 < p.num_kb) {
+          if (kb + 2 < kb1) {
             sa1 = __ldg(sap + (kb + 2) * p.sa_blk);
             sb1 = __ldg(sbp + (kb + 2) * p.sb_blk);
           }
@@ -339,6 +357,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           add(rb, 96);
         }
         if (!ok) break;
+        if constexpr (SPLIT) {  // there is a cluster for every tile
+          have = true;
+          break;
+        }
         if (p.bias != nullptr) {
 #pragma unroll
           for (int i = 0; i < 128; ++i)
@@ -387,6 +409,59 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         }
       }
       if (p.tma_out && lane == 0) bulk_wait_all0();  // this warp's TMA stores are complete before the CTA leaves
+      if constexpr (SPLIT) {
+        // the parts' sums through the idle rings, [256 columns][128 rows] fp32 each; part r adds and stores the groups
+        // r, r + split, ... of 16 columns, the parts in the order of K
+        __syncthreads();  // every load has landed and every MMA has read the ring
+        float* sums = reinterpret_cast<float*>(smem);
+        if (have) {
+#pragma unroll
+          for (int i = 0; i < 128; ++i) sums[(half * 128 + i) * BM + sub * 32 + lane] = acc[i];
+        }
+        __syncwarp();
+        cluster_sync();
+        const int64_t m = walk.lo + (2 * mb + crank) * BM + sub * 32 + lane;
+        if (have && m < walk.hi) {
+          for (int g = part + half * p.split; g < BN / 16; g += 2 * p.split) {
+            const int64_t n = static_cast<int64_t>(nb) * BN + 16 * g;
+            if (n >= p.N) break;
+            float v[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] = 0.0f;
+            for (int q = 0; q < p.split; ++q) {
+              const uint32_t src = mapa_shared(smem0 + static_cast<uint32_t>((16 * g * BM + sub * 32 + lane) * 4),
+                                               static_cast<uint32_t>(2 * q + crank));
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                float x;
+                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(src + 4u * BM * i) : "memory");
+                v[i] += x;
+              }
+            }
+            uint16_t* dst = p.y + m * p.ldy + n;
+            if (p.bias != nullptr) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                if (n + i < p.N) v[i] += __bfloat162float(p.bias[n + i]);
+            }
+#pragma unroll
+            for (int h8 = 0; h8 < 16; h8 += 8) {
+              if (p.vec_out && n + h8 + 8 <= p.N) {
+                *reinterpret_cast<uint4*>(dst + h8) =
+                    make_uint4(to_out2(v[h8], v[h8 + 1], p.out_f16), to_out2(v[h8 + 2], v[h8 + 3], p.out_f16),
+                               to_out2(v[h8 + 4], v[h8 + 5], p.out_f16), to_out2(v[h8 + 6], v[h8 + 7], p.out_f16));
+              } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                  if (n + h8 + i < p.N) dst[h8 + i] = to_out(v[h8 + i], p.out_f16);
+              }
+            }
+          }
+        }
+      }
+    } else if constexpr (SPLIT) {  // the barriers of the end phase
+      __syncthreads();
+      cluster_sync();
     }
   }
   __syncwarp();
@@ -404,49 +479,52 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 // ---------------------------------------------------------------------------------------------------------------
 namespace narrow {
 
-constexpr int THREADS = 192;    // producer, MMA issuer, 4 epilogue warps
-constexpr int CHUNK = 16;       // K steps whose scales are staged together
-constexpr int MAX_SPLIT = 8;
+constexpr int EPI_WARPS = 8, EPI_THREADS = 32 * EPI_WARPS;
+constexpr int THREADS = 64 + EPI_THREADS;  // producer, MMA issuer, epilogue (4 row quarters x 2 token halves)
+constexpr int CHUNK = 16;                  // K steps whose scales are staged together
+constexpr int MAX_SPLIT = 8, ROUND_COST = 20;
+constexpr int NBUF = 4;                    // TMEM buffers of NT columns: steps between the MMAs and the epilogue
 
 __host__ __device__ constexpr int stage_bytes(int nt) { return (BLK + nt) * BLK; }
-__host__ __device__ constexpr int stages(int nt) { return nt >= 128 ? 3 : 4; }
-// TMEM buffers of NT columns: 4 (a step of few tokens is short, so more of them are in flight), 2 for wide tiles
-__host__ __device__ constexpr int buffers(int nt) { return nt >= 64 ? 2 : 4; }
-// ring (reused for the sums that the cluster adds: NT x 128 fp32), barriers, two chunks of scales, alignment slack
+// two CTAs per SM with a ring of 4 each: more than the ~45 KB in flight that an SM's share of the memory bandwidth needs,
+// and one CTA's start and end lie under the other's loads
+constexpr int CTAS_PER_SM = 2, STAGES = 4;
+// ring (reused for the sums that the cluster adds: NT x 128 fp32), barriers, two chunks of scales, alignment slack; at
+// least a third of an SM's shared memory, so that no more than two CTAs fit and their TMEM never exceeds 512 columns (a
+// CTA that waited for TMEM while its cluster waits for it could wait forever)
 __host__ __device__ constexpr int smem(int nt) {
-  return stages(nt) * stage_bytes(nt) + 256 + 2 * CHUNK * nt * 4 + 1024;
+  const int need = STAGES * stage_bytes(nt) + 256 + 2 * CHUNK * nt * 4 + 1024;
+  return need < 79 * 1024 ? 79 * 1024 : need;
 }
-// TMEM is never oversubscribed (a CTA that waited for TMEM while its cluster waits for it could wait forever): at most
-// 232448 / smem CTAs fit on an SM, and that many allocations fit in its 512 columns
-__host__ __device__ constexpr bool tmem_fits(int nt) { return (233472 / (smem(nt) + 1024)) * (buffers(nt) * nt) <= 512; }
-static_assert(tmem_fits(16) && tmem_fits(32) && tmem_fits(64) && tmem_fits(128), "TMEM columns");
-static_assert(stages(128) * stage_bytes(128) >= 128 * BLK * 4 && stages(16) * stage_bytes(16) >= 16 * BLK * 4 &&
-              stages(64) * stage_bytes(64) >= 64 * BLK * 4, "the ring holds the sums");
+__host__ __device__ constexpr bool tmem_fits(int nt) { return (233472 / (smem(nt) + 1024)) * (NBUF * nt) <= 512; }
+static_assert(tmem_fits(16) && tmem_fits(32) && tmem_fits(64), "TMEM columns");
+static_assert(STAGES * stage_bytes(64) >= 64 * BLK * 4 && smem(64) + 1024 <= 233472 / CTAS_PER_SM, "shared memory");
 
 template <int NT>
-__global__ void __launch_bounds__(THREADS, 2) kernel(const __grid_constant__ CUtensorMap tmA,
-                                                     const __grid_constant__ CUtensorMap tmW,
-                                                     const __grid_constant__ Params p) {
-  constexpr int STAGES = stages(NT), STAGE_BYTES = stage_bytes(NT), NBUF = buffers(NT);
+__global__ void __launch_bounds__(THREADS, CTAS_PER_SM) kernel(const __grid_constant__ CUtensorMap tmA,
+                                                                   const __grid_constant__ CUtensorMap tmW,
+                                                                   const __grid_constant__ Params p) {
+  constexpr int STAGE_BYTES = stage_bytes(NT);
+  constexpr int MINE = NT / 2;  // tokens of an epilogue thread
   constexpr uint32_t TMEM_COLS = NBUF * NT, IDESC = idesc_make(FMT_E4M3, FMT_E4M3, 0, 128, NT);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE_BYTES);
-  // bars: full[STAGES], empty[STAGES], tfull[NBUF], tempty[NBUF], done; then the TMEM address and the start flag
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 2 * NBUF + 1);
+  // bars: full[STAGES], used[STAGES], tempty[NBUF], done; then the TMEM address and the start flag.  used[s]: the MMAs of
+  // the step in stage s are complete, for the producer and for the epilogue.
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + NBUF + 1);
   uint32_t* start_flag = tmem_slot + 1;
   float* scales = reinterpret_cast<float*>(smem + STAGES * STAGE_BYTES + 256);  // [2][CHUNK][NT]
   float* sums = reinterpret_cast<float*>(smem);                                 // [NT][128] once the ring is idle
-  static_assert(8 * (2 * STAGES + 2 * NBUF + 1) + 8 <= 256, "barrier area");
+  static_assert(8 * (2 * STAGES + NBUF + 1) + 8 <= 256, "barrier area");
   const uint32_t smem0 = smem_u32(smem), bar0 = smem_u32(bars);
   auto full_bar = [&](int s) { return bar0 + 8u * s; };
-  auto empty_bar = [&](int s) { return bar0 + 8u * (STAGES + s); };
-  auto tfull_bar = [&](int b) { return bar0 + 8u * (2 * STAGES + b); };
-  auto tempty_bar = [&](int b) { return bar0 + 8u * (2 * STAGES + NBUF + b); };
-  const uint32_t done_bar = bar0 + 8u * (2 * STAGES + 2 * NBUF);
+  auto used_bar = [&](int s) { return bar0 + 8u * (STAGES + s); };
+  auto tempty_bar = [&](int b) { return bar0 + 8u * (2 * STAGES + b); };
+  const uint32_t done_bar = bar0 + 8u * (2 * STAGES + NBUF);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int split = static_cast<int>(gridDim.x) / p.num_nb;  // CTAs of the cluster: they share blockIdx.x / split
+  const int split = p.split;  // CTAs of the cluster: they share blockIdx.x / split
   const int crank = static_cast<int>(blockIdx.x) % split, nb = static_cast<int>(blockIdx.x) / split;
   Walk<NT> walk;
   const bool found = walk.find(p, blockIdx.y, 1);  // the same for every CTA of the cluster
@@ -461,12 +539,9 @@ __global__ void __launch_bounds__(THREADS, 2) kernel(const __grid_constant__ CUt
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(full_bar(s), 1);
-      mbar_init(empty_bar(s), 1);
+      mbar_init(used_bar(s), 1);
     }
-    for (int b = 0; b < NBUF; ++b) {
-      mbar_init(tfull_bar(b), 1);
-      mbar_init(tempty_bar(b), 4);
-    }
+    for (int b = 0; b < NBUF; ++b) mbar_init(tempty_bar(b), EPI_WARPS);
     mbar_init(done_bar, 1);
     fence_mbar_init();
     *start_flag = status_bad(p.wc) ? 0u : 1u;
@@ -480,23 +555,23 @@ __global__ void __launch_bounds__(THREADS, 2) kernel(const __grid_constant__ CUt
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   const bool start = cluster_flag(smem_u32(start_flag));
-  float acc[NT];
+  float acc[MINE];
 #pragma unroll
-  for (int i = 0; i < NT; ++i) acc[i] = 0.0f;
+  for (int i = 0; i < MINE; ++i) acc[i] = 0.0f;
 
   if (start) {
     if (warp == 0) {
       if (lane == 0) {
-        uint32_t used = 0, last = 0;
+        uint32_t loaded = 0, last = 0;
         int stage = 0;
         uint32_t phase = 0;
         for (int kb = kb0; kb < kb1; ++kb) {
-          if (!mbar_wait(empty_bar(stage), phase ^ 1u, p.wc)) break;
+          if (!mbar_wait(used_bar(stage), phase ^ 1u, p.wc)) break;
           const uint32_t sW = smem0 + stage * STAGE_BYTES;
           mbar_arrive_expect_tx(full_bar(stage), STAGE_BYTES);
           tma_load_3d(sW, &tmW, full_bar(stage), kb * BLK, nb * BLK, walk.e);
           tma_load_2d(sW + BLK * BLK, &tmA, full_bar(stage), kb * BLK, static_cast<int32_t>(t0));
-          used |= 1u << stage;
+          loaded |= 1u << stage;
           last = (last & ~(1u << stage)) | (phase << stage);
           if (++stage == STAGES) {
             stage = 0;
@@ -504,7 +579,7 @@ __global__ void __launch_bounds__(THREADS, 2) kernel(const __grid_constant__ CUt
           }
         }
         for (int s = 0; s < STAGES; ++s) {  // no TMA write in flight when the ring is given up
-          if (!(used >> s & 1u)) continue;
+          if (!(loaded >> s & 1u)) continue;
           const uint64_t c0 = globaltimer();
           while (!mbar_try_wait(full_bar(s), last >> s & 1u) && globaltimer() - c0 < p.wc.timeout) {
           }
@@ -516,15 +591,14 @@ __global__ void __launch_bounds__(THREADS, 2) kernel(const __grid_constant__ CUt
         uint32_t phase = 0, it = 0;
         for (int kb = kb0; kb < kb1; ++kb, ++it) {
           const int b = it % NBUF;
-          if (!mbar_wait(tempty_bar(b), ((it / NBUF) & 1u) ^ 1u, p.wc) || !mbar_wait(full_bar(stage), phase, p.wc)) break;
+          if (!mbar_wait(full_bar(stage), phase, p.wc) || !mbar_wait(tempty_bar(b), ((it / NBUF) & 1u) ^ 1u, p.wc)) break;
           tc_fence_after();
           const uint32_t sW = smem0 + stage * STAGE_BYTES;
           const uint64_t wdesc = sdesc_sw128(sW, 16, 1024), adesc = sdesc_sw128(sW + BLK * BLK, 16, 1024);
 #pragma unroll
           for (int kk = 0; kk < BLK / 32; ++kk)
             umma_f8_ss(tmem_base + static_cast<uint32_t>(b * NT), wdesc + 2u * kk, adesc + 2u * kk, IDESC, kk != 0);
-          umma_commit(tfull_bar(b));
-          umma_commit(empty_bar(stage));
+          umma_commit(used_bar(stage));
           if (++stage == STAGES) {
             stage = 0;
             phase ^= 1u;
@@ -536,62 +610,71 @@ __global__ void __launch_bounds__(THREADS, 2) kernel(const __grid_constant__ CUt
         }
       }
     } else {
-      // ---------------- epilogue: thread = weight row, NT running sums ----------------
-      const int sub = warp & 3, tid = threadIdx.x - 64;
-      const uint32_t tmine = tmem_base + (static_cast<uint32_t>(sub * 32) << 16);
+      // ---------------- epilogue: thread = weight row and half of the tokens ----------------
+      const int sub = warp & 3, half = (warp - 2) >> 2, tid = threadIdx.x - 64;
+      const uint32_t tmine = tmem_base + (static_cast<uint32_t>(sub * 32) << 16) + static_cast<uint32_t>(half * MINE);
       const float* sbp = p.sb + walk.e * p.sb_exp + nb * p.sb_row;
-      // sa * sb of a chunk of steps for the tile's tokens; thread tid holds values tid, tid + 128, ... of [CHUNK][NT]
-      constexpr int PER = CHUNK * NT / 128;
+      // sa * sb of a chunk of steps for the tile's tokens; thread tid holds values tid, tid + 256, ... of [CHUNK][NT]
+      constexpr int PER = CHUNK * NT / EPI_THREADS;
       float next[PER];
       auto fetch = [&](int kb) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-          const int v = tid + 128 * i, k = kb + v / NT, tok = v % NT;
+          const int v = tid + EPI_THREADS * i, k = kb + v / NT, tok = v % NT;
           next[i] = (k < kb1 && t0 + tok < walk.hi)
                         ? __ldg(p.sa + (t0 + tok) * p.sa_row + k * p.sa_blk) * __ldg(sbp + k * p.sb_blk)
                         : 0.0f;
         }
       };
       fetch(kb0);
-      uint32_t it = 0;
+      uint32_t it = 0, phase = 0;
+      int stage = 0;
       bool ok = true;
-      // every thread of the 128 takes the barrier of each chunk, also after a wait that gave up
+      // every epilogue thread takes the barrier of each chunk, also after a wait that gave up
       for (int c0 = kb0; c0 < kb1; c0 += CHUNK) {
         float* sc = scales + (((c0 - kb0) / CHUNK) & 1) * CHUNK * NT;
 #pragma unroll
-        for (int i = 0; i < PER; ++i) sc[tid + 128 * i] = next[i];
-        asm volatile("bar.sync 1, 128;" ::: "memory");
+        for (int i = 0; i < PER; ++i) sc[tid + EPI_THREADS * i] = next[i];
+        asm volatile("bar.sync 1, %0;" ::"n"(EPI_THREADS) : "memory");
         if (c0 + CHUNK < kb1) fetch(c0 + CHUNK);
         const int c1 = min(c0 + CHUNK, kb1);
+        const float* s = sc + half * MINE;
 #pragma unroll 1
-        for (int kb = c0; kb < c1; ++kb, ++it) {
+        for (int kb = c0; kb < c1; ++kb, ++it, s += NT) {
           const int b = it % NBUF;
-          ok = __all_sync(0xffffffffu, ok && mbar_wait(tfull_bar(b), (it / NBUF) & 1u, p.wc));
+          ok = __all_sync(0xffffffffu, ok && mbar_wait(used_bar(stage), phase, p.wc));
           if (!ok) break;
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
           tc_fence_after();
-          const float* s = sc + (kb - c0) * NT;
-          constexpr int W = NT == 32 || NT == 64 ? 32 : 16;
+          const uint32_t tcur = tmine + static_cast<uint32_t>(b * NT);
+          constexpr int W = MINE < 16 ? MINE : 16;
 #pragma unroll
-          for (int c = 0; c < NT / W; ++c) {
+          for (int c = 0; c < MINE; c += W) {
             uint32_t r[W];
-            if constexpr (W == 16)
-              tmem_ld16(tmine + static_cast<uint32_t>(b * NT + c * 16), r);
+            if constexpr (W == 8)
+              tmem_ld8(tcur, r);
             else
-              tmem_ld32(tmine + static_cast<uint32_t>(b * NT + c * 32), r);
+              tmem_ld16(tcur + c, r);
             tmem_ld_wait();
-            reg_fence(r);
-            if (c == NT / W - 1) {
+            if constexpr (W >= 16)
+              reg_fence(r);
+            else
+              asm volatile("" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]));
+            if (c + W == MINE) {
               tc_fence_before();
               __syncwarp();
               if (lane == 0) mbar_arrive(tempty_bar(b));
             }
 #pragma unroll
             for (int i = 0; i < W; i += 4) {
-              const float4 f = *reinterpret_cast<const float4*>(s + c * W + i);
-              acc[c * W + i] = fmaf(__uint_as_float(r[i]), f.x, acc[c * W + i]);
-              acc[c * W + i + 1] = fmaf(__uint_as_float(r[i + 1]), f.y, acc[c * W + i + 1]);
-              acc[c * W + i + 2] = fmaf(__uint_as_float(r[i + 2]), f.z, acc[c * W + i + 2]);
-              acc[c * W + i + 3] = fmaf(__uint_as_float(r[i + 3]), f.w, acc[c * W + i + 3]);
+              const float4 f = *reinterpret_cast<const float4*>(s + c + i);
+              acc[c + i] = fmaf(__uint_as_float(r[i]), f.x, acc[c + i]);
+              acc[c + i + 1] = fmaf(__uint_as_float(r[i + 1]), f.y, acc[c + i + 1]);
+              acc[c + i + 2] = fmaf(__uint_as_float(r[i + 2]), f.z, acc[c + i + 2]);
+              acc[c + i + 3] = fmaf(__uint_as_float(r[i + 3]), f.w, acc[c + i + 3]);
             }
           }
         }
@@ -600,27 +683,29 @@ __global__ void __launch_bounds__(THREADS, 2) kernel(const __grid_constant__ CUt
   }
   __syncwarp();
   __syncthreads();  // the ring is idle: every load has landed and every MMA has read it
-  const int64_t n = static_cast<int64_t>(nb) * BLK + (warp & 3) * 32 + lane;
+  const int col = (warp & 3) * 32 + lane;
+  const int64_t n = static_cast<int64_t>(nb) * BLK + col;
   const bool epi = warp >= 2;
+  const int first = epi ? (warp - 2) / 4 * MINE : 0;  // the thread's first token
   const float bias = epi && p.bias != nullptr && n < p.N ? __bfloat162float(p.bias[n]) : 0.0f;
   const int tokens = static_cast<int>(walk.hi - t0 < NT ? walk.hi - t0 : NT);
   if (split == 1) {
     if (epi && start && n < p.N) {
 #pragma unroll
-      for (int i = 0; i < NT; ++i)
-        if (i < tokens) p.y[(t0 + i) * p.ldy + n] = to_out(acc[i] + bias, p.out_f16);
+      for (int i = 0; i < MINE; ++i)
+        if (first + i < tokens) p.y[(t0 + first + i) * p.ldy + n] = to_out(acc[i] + bias, p.out_f16);
     }
   } else {
-    const int col = (warp & 3) * 32 + lane;
     if (epi) {
 #pragma unroll
-      for (int i = 0; i < NT; ++i) sums[i * BLK + col] = acc[i];
+      for (int i = 0; i < MINE; ++i) sums[(first + i) * BLK + col] = acc[i];
     }
     __syncwarp();
     cluster_sync();
     if (epi && start && n < p.N) {
-      // CTA r of the cluster adds and stores tokens r, r + split, ...: the parts in the order of K
-      for (int i = crank; i < tokens; i += split) {
+      // CTA r of the cluster adds and stores tokens r, r + split, ... (its two warp groups in turn): parts in the order
+      // of K
+      for (int i = crank + split * ((warp - 2) / 4); i < tokens; i += 2 * split) {
         float v = 0.0f;
         for (int q = 0; q < split; ++q) {
           float part;
@@ -663,62 +748,112 @@ int weight_map(CUtensorMap* map, const void* base, int64_t K, int64_t N, int64_t
   return encode_tmap(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-int launch_wide(Params& p, const CUtensorMap& tmA, const CUtensorMap& tmW, int64_t tiles, int dev, cudaStream_t st) {
-  static std::atomic<int> fit_of[MAX_DEVICES];
-  int fit = fit_of[dev].load(std::memory_order_acquire);
-  if (fit == 0) {
-    cudaError_t e = cudaFuncSetAttribute(wide::kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, wide::SMEM);
-    if (e == cudaSuccess) {
-      cudaLaunchConfig_t cfg = {};
-      cfg.gridDim = dim3(static_cast<unsigned>(num_sms() & ~1), 1, 1);
-      cfg.blockDim = dim3(wide::THREADS, 1, 1);
-      cfg.dynamicSmemBytes = wide::SMEM;
-      e = cudaOccupancyMaxActiveClusters(&fit, wide::kernel, &cfg);
-    }
-    if (e != cudaSuccess) return cuda_fail(e, "fp8_gemm_blocks: shared memory / cluster occupancy");
-    if (fit < 1) return fail(H3B_EUNSUPPORTED, "fp8_gemm_blocks: no CTA pair fits on this device");
-    fit_of[dev].store(fit, std::memory_order_release);
+int launch(const void* kernel, dim3 grid, int threads, int smem, int cluster, void** args, cudaStream_t st, int* fit) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  // with `fit`: no launch, but how many such clusters run at once
+  const cudaError_t e = fit != nullptr ? cudaOccupancyMaxActiveClusters(fit, kernel, &cfg) : cudaLaunchKernelExC(&cfg, kernel, args);
+  if (e != cudaSuccess) return cuda_fail(e, fit != nullptr ? "fp8_gemm_blocks: cluster occupancy" : "fp8_gemm_blocks launch");
+  return H3B_OK;
+}
+
+// How many clusters of 1 .. MAX parts (of `unit` CTAs each) run at once on a device: looked up once, -1 for none.  The
+// query counts one CTA per SM for a kernel that allocates TMEM; `per_sm` do run together (measured: CTAs of 64 columns).
+template <int MAX>
+struct Fit {
+  std::atomic<int> of[MAX_DEVICES][MAX];
+  int get(const void* kernel, int threads, int smem, int unit, int per_sm, int dev, int parts, int* fit) {
+    *fit = of[dev][parts - 1].load(std::memory_order_acquire);
+    if (*fit != 0) return H3B_OK;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    // without this the SM's shared memory is set up for a single CTA
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    if (e != cudaSuccess) return cuda_fail(e, "fp8_gemm_blocks: shared memory");
+    const int cluster = unit * parts;
+    const int rc = launch(kernel, dim3(static_cast<unsigned>(cluster * num_sms()), 1, 1), threads, smem, cluster, nullptr, nullptr, fit);
+    if (rc) return rc;
+    *fit *= per_sm;
+    if (*fit < 1) *fit = -1;
+    of[dev][parts - 1].store(*fit, std::memory_order_release);
+    return H3B_OK;
   }
+};
+
+// The number of parts of K (clusters of parts * unit CTAs, a tile each) that ends first: rounds of tiles times the steps of
+// a part and `round_cost`, what a round takes besides, in steps.  A persistent grid of single parts pays that once.
+// `whole` / `parts`: the kernels for one part and for more.
+template <int MAX>
+int pick_split(Fit<MAX>& fits, const void* whole, const void* parts, int threads, int smem, int unit, int per_sm, int dev, int64_t tiles, int num_kb,
+               int round_cost, bool persistent, int* split, int* fit1) {
+  double best = 0;
+  for (int s = 1; s <= MAX; ++s) {
+    if (s > 1 && num_kb < 4 * s) break;  // four steps each at least
+    int fit = 0;
+    const int rc = fits.get(s == 1 ? whole : parts, threads, smem, unit, per_sm, dev, s, &fit);
+    if (rc) return rc;
+    if (s == 1) {
+      if (fit < 1) return fail(H3B_EUNSUPPORTED, "fp8_gemm_blocks: the kernel does not fit on this device");
+      *fit1 = fit;
+    }
+    if (fit < 1) continue;
+    const double rounds = static_cast<double>((tiles + fit - 1) / fit);
+    const double steps = static_cast<double>((num_kb + s - 1) / s);
+    const double cost = s == 1 && persistent ? rounds * steps + round_cost : rounds * (steps + round_cost);
+    if (s == 1 || cost < best) {
+      best = cost;
+      *split = s;
+    }
+  }
+  return H3B_OK;
+}
+
+int launch_wide(Params& p, const CUtensorMap& tmA, const CUtensorMap& tmW, int64_t tiles, int64_t expected, int dev,
+                cudaStream_t st) {
+  static Fit<wide::MAX_SPLIT> fits;
+  const void* whole = reinterpret_cast<const void*>(wide::kernel<false>);
+  const void* parts = reinterpret_cast<const void*>(wide::kernel<true>);
+  int fit = 0;
+  int rc = pick_split(fits, whole, parts, wide::THREADS, wide::SMEM, 2, 1, dev, expected, p.num_kb, wide::ROUND_COST, true, &p.split, &fit);
+  if (rc) return rc;
   CUtensorMap tmY = tmA;  // a valid map where no TMA store is made
   p.vec_out = al16(p.y) && p.ldy % 8 == 0;
   if (p.vec_out) {
     const uint64_t dims[2] = {static_cast<uint64_t>(p.N), static_cast<uint64_t>(p.T)};
     const uint64_t strides[1] = {static_cast<uint64_t>(p.ldy) * 2};
     const uint32_t box[2] = {64, 32};
-    const int rc = encode_tmap(&tmY, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, p.y, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    rc = encode_tmap(&tmY, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, p.y, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc) return rc;
     p.tma_out = 1;
   }
-  const int grid = 2 * static_cast<int>(tiles < fit ? tiles : fit);
-  wide::kernel<<<grid, wide::THREADS, wide::SMEM, st>>>(tmA, tmW, tmY, p);
-  H3B_CHECK_LAUNCH("fp8_gemm_blocks launch");
-  return H3B_OK;
+  // one part: as many pairs as run at once walk the tiles; more: a cluster for every tile that there can be
+  const int64_t clusters = p.split == 1 && tiles > fit ? fit : tiles;
+  void* args[] = {const_cast<CUtensorMap*>(&tmA), const_cast<CUtensorMap*>(&tmW), &tmY, &p};
+  return launch(p.split == 1 ? whole : parts, dim3(static_cast<unsigned>(2 * p.split * clusters), 1, 1), wide::THREADS, wide::SMEM, 2 * p.split, args,
+                st, nullptr);
 }
 
 template <int NT>
-int launch_narrow(const Params& p, const CUtensorMap& tmA, const CUtensorMap& tmW, int64_t token_tiles, int split, int dev,
-                  cudaStream_t st) {
-  static std::atomic<int> ready[MAX_DEVICES];
-  if (!ready[dev].load(std::memory_order_acquire)) {
-    const cudaError_t e = cudaFuncSetAttribute(narrow::kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, narrow::smem(NT));
-    if (e != cudaSuccess) return cuda_fail(e, "fp8_gemm_blocks: shared memory");
-    ready[dev].store(1, std::memory_order_release);
-  }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(p.num_nb * split), static_cast<unsigned>(token_tiles), 1);
-  cfg.blockDim = dim3(narrow::THREADS, 1, 1);
-  cfg.dynamicSmemBytes = narrow::smem(NT);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = static_cast<unsigned>(split);
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, narrow::kernel<NT>, tmA, tmW, p);
-  if (e != cudaSuccess) return cuda_fail(e, "fp8_gemm_blocks launch");
-  return H3B_OK;
+int launch_narrow(Params& p, const CUtensorMap& tmA, const CUtensorMap& tmW, int64_t token_tiles, int dev, cudaStream_t st) {
+  static Fit<narrow::MAX_SPLIT> fits;
+  const void* kernel = reinterpret_cast<const void*>(narrow::kernel<NT>);
+  int fit = 0;
+  const int rc = pick_split(fits, kernel, kernel, narrow::THREADS, narrow::smem(NT), 1, narrow::CTAS_PER_SM, dev, token_tiles * p.num_nb, p.num_kb,
+                            narrow::ROUND_COST, false, &p.split, &fit);
+  if (rc) return rc;
+  void* args[] = {const_cast<CUtensorMap*>(&tmA), const_cast<CUtensorMap*>(&tmW), &p};
+  return launch(kernel, dim3(static_cast<unsigned>(p.num_nb * p.split), static_cast<unsigned>(token_tiles), 1),
+                narrow::THREADS, narrow::smem(NT), p.split, args, st, nullptr);
 }
 
 struct Operands {
@@ -787,29 +922,26 @@ int gemm_blocks(const char* what, const Operands& o, cudaStream_t st) {
   // groups that can hold a row, and the row tiles that they can need at most
   const int64_t active = o.T < o.E ? o.T : o.E;
   const int64_t mean = (o.T + o.E - 1) / o.E;
-  if (mean > 128) {
+  if (mean > 64) {
     p.num_nb = static_cast<int>((o.N + wide::BN - 1) / wide::BN);
     const int64_t tiles = (o.T + active * (2 * wide::BM - 1)) / (2 * wide::BM) * p.num_nb;
-    if (tiles > most) return fail(H3B_EUNSUPPORTED, "%s: 2^31 tiles or more", what);
+    if (tiles > most / (2 * wide::MAX_SPLIT)) return fail(H3B_EUNSUPPORTED, "%s: 2^31 tiles or more", what);
     rc = load_map(&tmA, o.a, o.K, o.T, o.lda, wide::BM);
     if (rc) return rc;
-    return launch_wide(p, tmA, tmW, tiles, dev, st);
+    // the tiles to expect: rows / 256 and, where there are several groups, half a row block more for each
+    const int64_t expected = o.E == 1 ? tiles : (o.T + active * wide::BM) / (2 * wide::BM) * p.num_nb;
+    return launch_wide(p, tmA, tmW, tiles, expected < 1 ? 1 : expected, dev, st);
   }
-  const int nt = mean <= 16 ? 16 : (mean <= 32 ? 32 : (mean <= 64 ? 64 : 128));
+  const int nt = mean <= 16 ? 16 : (mean <= 32 ? 32 : 64);
   p.num_nb = static_cast<int>((o.N + BLK - 1) / BLK);
   const int64_t token_tiles = (o.T + active * (nt - 1)) / nt;
   if (token_tiles > 65535) return fail(H3B_EUNSUPPORTED, "%s: %lld row tiles", what, (long long)token_tiles);
-  int split = 1;
-  while (split < narrow::MAX_SPLIT && token_tiles * p.num_nb * split < 2 * num_sms() && p.num_kb >= 8 * split) split *= 2;
-  if (static_cast<int64_t>(p.num_nb) * split > most) return fail(H3B_EUNSUPPORTED, "%s: 2^31 tiles or more", what);
+  if (static_cast<int64_t>(p.num_nb) * narrow::MAX_SPLIT > most) return fail(H3B_EUNSUPPORTED, "%s: 2^31 tiles or more", what);
   rc = load_map(&tmA, o.a, o.K, o.T, o.lda, static_cast<uint32_t>(nt));
   if (rc) return rc;
-  switch (nt) {
-    case 16: return launch_narrow<16>(p, tmA, tmW, token_tiles, split, dev, st);
-    case 32: return launch_narrow<32>(p, tmA, tmW, token_tiles, split, dev, st);
-    case 64: return launch_narrow<64>(p, tmA, tmW, token_tiles, split, dev, st);
-    default: return launch_narrow<128>(p, tmA, tmW, token_tiles, split, dev, st);
-  }
+  if (nt == 16) return launch_narrow<16>(p, tmA, tmW, token_tiles, dev, st);
+  if (nt == 32) return launch_narrow<32>(p, tmA, tmW, token_tiles, dev, st);
+  return launch_narrow<64>(p, tmA, tmW, token_tiles, dev, st);
 }
 
 }  // namespace

@@ -26,7 +26,8 @@ def _need_cuda(*ts: torch.Tensor | None) -> None:
 
 
 def _stream(t: torch.Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
+    # the raw handle: building a torch.cuda.Stream object for it costs more than a small kernel's launch
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
 
 
 def _ptr(t: torch.Tensor | None) -> int | None:
@@ -466,35 +467,32 @@ def _nblocks(n: int) -> int:
 
 def _launch(ref: torch.Tensor, name: str, *args) -> None:
     """Call ``name`` with ``ref``'s device current, on that device's current torch stream."""
-    dev = ref.device.index
-    if dev is None or dev == torch.cuda.current_device():
+    dev = ref.get_device()
+    if dev < 0 or dev == torch._C._cuda_getDevice():
         _lib.call(name, *args, _stream(ref))
         return
     with torch.cuda.device(dev):
         _lib.call(name, *args, _stream(ref))
 
 
-def _one_device(ref: torch.Tensor, what: str, *ts: torch.Tensor | None) -> None:
-    _need_cuda(ref, *ts)
-    for t in ts:
-        if t is not None and t.device != ref.device:
-            raise ValueError(f"{what}: tensors on {ref.device} and {t.device}")
-
-
-def _unit_rows(t: torch.Tensor, dtype: torch.dtype, dims: int, what: str) -> None:
-    """A ``dims``-dimensional tensor of ``dtype`` whose rows are dense (unit innermost stride)."""
+def _unit_rows(t: torch.Tensor, dtype: torch.dtype, dims: int, what: str) -> tuple[int, ...]:
+    """The strides of a ``dims``-dimensional tensor of ``dtype`` whose rows are dense (unit innermost stride)."""
     if t.dtype != dtype:
         raise TypeError(f"{what}: dtype {t.dtype}, expected {dtype}")
-    if t.dim() != dims or (t.stride(-1) != 1 and t.shape[-1] > 1):
+    strides = t.stride()
+    if len(strides) != dims or (strides[-1] != 1 and t.shape[-1] > 1):
         raise ValueError(f"{what}: must have {dims} dimensions and unit innermost stride, got {tuple(t.shape)} with "
-                         f"strides {t.stride()}")
+                         f"strides {strides}")
+    return strides
 
 
-def _row_scales(rows: int, cols: int, like: torch.Tensor) -> torch.Tensor:
-    """Scales [rows, ceil(cols / 128)] stored block by block (strides (1, rows rounded up to 4)): a tile's row scales of
-    one block are then consecutive in memory, which is how the products read them."""
-    return torch.empty_strided((rows, _nblocks(cols)), (1, max(rows + 3 & ~3, 4)), dtype=torch.float32,
-                               device=like.device)
+def _quant_outputs(rows: int, cols: int, device: torch.device) -> tuple[torch.Tensor, torch.Tensor, int]:
+    """q [rows, cols] e4m3 contiguous and scales [rows, ceil(cols / 128)] stored block by block, and the stride between
+    blocks (rows rounded up to 4): a tile's row scales of one block are then consecutive in memory, which is how the
+    products read them.  (``empty_strided`` parses its arguments in half the time of ``empty``.)"""
+    ld = max(rows + 3 & ~3, 4)
+    q = torch.empty_strided((rows, cols), (cols, 1), dtype=E4M3, device=device)
+    return q, torch.empty_strided((rows, -(-cols // BLOCK)), (1, ld), dtype=torch.float32, device=device), ld
 
 
 def quant_blocks(h: torch.Tensor, *, div_mode: int = DIV_IEEE) -> tuple[torch.Tensor, torch.Tensor]:
@@ -502,12 +500,10 @@ def quant_blocks(h: torch.Tensor, *, div_mode: int = DIV_IEEE) -> tuple[torch.Te
     fp32), the per-token quant's scale and rounding taken over each 128 columns.  The scale tensor is stored block by
     block (unit stride along M)."""
     _need_cuda(h)
-    _unit_rows(h, torch.bfloat16, 2, "quant_blocks h")
+    ld = _unit_rows(h, torch.bfloat16, 2, "quant_blocks h")[0]
     m, k = h.shape
-    q = torch.empty((m, k), dtype=E4M3, device=h.device)
-    s = _row_scales(m, k, h)
-    _launch(h, "h3b_quant_blocks_e4m3", h.data_ptr(), m, k, h.stride(0), q.data_ptr(), s.data_ptr(), s.stride(0),
-            s.stride(1), div_mode)
+    q, s, s_blk = _quant_outputs(m, k, h.device)
+    _launch(h, "h3b_quant_blocks_e4m3", h.data_ptr(), m, k, ld, q.data_ptr(), s.data_ptr(), 1, s_blk, div_mode)
     return q, s
 
 
@@ -515,14 +511,13 @@ def silu_mul_quant_blocks(x: torch.Tensor, *, div_mode: int = DIV_IEEE) -> tuple
     """silu(gate) * up of bf16 x [M, 2F] (gate columns, then up columns), in fp32, then the block quant: (q [M, F] e4m3,
     scale [M, ceil(F/128)] fp32).  The product is not rounded to bf16 in between (``silu_mul_quant`` does)."""
     _need_cuda(x)
-    _unit_rows(x, torch.bfloat16, 2, "silu_mul_quant_blocks x")
+    ld = _unit_rows(x, torch.bfloat16, 2, "silu_mul_quant_blocks x")[0]
     m, width = x.shape
     if width % 2:
         raise ValueError(f"silu_mul_quant_blocks: x must be [rows, 2F], got {tuple(x.shape)}")
-    q = torch.empty((m, width // 2), dtype=E4M3, device=x.device)
-    s = _row_scales(m, width // 2, x)
-    _launch(x, "h3b_silu_mul_quant_blocks_e4m3", x.data_ptr(), m, width // 2, x.stride(0), q.data_ptr(), s.data_ptr(),
-            s.stride(0), s.stride(1), div_mode)
+    f = width // 2
+    q, s, s_blk = _quant_outputs(m, f, x.device)
+    _launch(x, "h3b_silu_mul_quant_blocks_e4m3", x.data_ptr(), m, f, ld, q.data_ptr(), s.data_ptr(), 1, s_blk, div_mode)
     return q, s
 
 
@@ -532,45 +527,54 @@ def quant_weight_blocks(w: torch.Tensor, *, div_mode: int = DIV_IEEE) -> tuple[t
     _need_cuda(w)
     if w.dim() not in (2, 3):
         raise ValueError(f"quant_weight_blocks: w must be [N, K] or [E, N, K], got {tuple(w.shape)}")
-    _unit_rows(w, torch.bfloat16, w.dim(), "quant_weight_blocks w")
+    strides = _unit_rows(w, torch.bfloat16, w.dim(), "quant_weight_blocks w")
     n, k = w.shape[-2:]
     e = w.shape[0] if w.dim() == 3 else 1
     q = torch.empty(w.shape, dtype=E4M3, device=w.device)
     s = torch.empty((*w.shape[:-2], _nblocks(n), _nblocks(k)), dtype=torch.float32, device=w.device)
-    _launch(w, "h3b_quant_weight_blocks_e4m3", w.data_ptr(), e, n, k, w.stride(0) if w.dim() == 3 else 0, w.stride(-2),
+    _launch(w, "h3b_quant_weight_blocks_e4m3", w.data_ptr(), e, n, k, strides[0] if w.dim() == 3 else 0, strides[-2],
             q.data_ptr(), s.data_ptr(), div_mode)
     return q, s
 
 
-def _block_product(a, w, sa, sb, bias, out_dtype, out, what: str, offsets=None):  # noqa: ANN001,ANN202
-    """The arguments that both block-scaled products share, checked; returns the output tensor."""
-    _one_device(a, what, w, sa, sb, bias, offsets, out)
-    _unit_rows(a, E4M3, 2, f"{what} a")
-    _unit_rows(w, E4M3, 2 if offsets is None else 3, f"{what} w")
+def _product_operands(a, w, sa, sb, others, out_dtype, out, what: str, dims: int):  # noqa: ANN001,ANN202
+    """The operands that both block-scaled products share (w and sb of ``dims`` dimensions), checked.  Returns (m, n, k,
+    row stride of a, strides of w, output, its row stride)."""
+    device = a.device
+    for t in (a, w, sa, sb, out, *others):
+        if t is not None:
+            _need_cuda(t)
+            if t.device != device:
+                raise ValueError(f"{what}: tensors on {device} and {t.device}")
+    sa_t, sb_t = sa.dtype, sb.dtype
+    lda = _unit_rows(a, E4M3, 2, f"{what} a")[0]
+    w_strides = _unit_rows(w, E4M3, dims, f"{what} w")
     m, k = a.shape
-    n = w.shape[-2]
-    if w.shape[-1] != k or k < 16 or k % 16 or n < 1:
+    *lead, n, k_w = w.shape
+    if k_w != k or k < 16 or k % 16 or n < 1:
         raise ValueError(f"{what}: a {tuple(a.shape)} and w {tuple(w.shape)} need the same K, a multiple of 16")
-    if sa.dtype != torch.float32 or sb.dtype != torch.float32:
-        raise TypeError(f"{what}: scales must be fp32, got {sa.dtype} and {sb.dtype}")
-    kb = _nblocks(k)
-    if tuple(sa.shape) != (m, kb) or tuple(sb.shape) != (*w.shape[:-2], _nblocks(n), kb):
-        raise ValueError(f"{what}: sa must be {(m, kb)} and sb {(*w.shape[:-2], _nblocks(n), kb)}, got "
-                         f"{tuple(sa.shape)} and {tuple(sb.shape)}")
+    if sa_t != torch.float32 or sb_t != torch.float32:
+        raise TypeError(f"{what}: scales must be fp32, got {sa_t} and {sb_t}")
+    kb = -(-k // BLOCK)
+    if sa.shape != (m, kb) or sb.shape != (*lead, -(-n // BLOCK), kb):
+        raise ValueError(f"{what}: sa must be {(m, kb)} and sb {(*lead, _nblocks(n), kb)}, got {tuple(sa.shape)} and "
+                         f"{tuple(sb.shape)}")
     if out is None:
         if out_dtype not in (torch.bfloat16, torch.float16):
             raise TypeError(f"{what}: out_dtype {out_dtype}, expected bf16 or f16")
-        return torch.empty((m, n), dtype=out_dtype, device=a.device)
-    _dt(out, torch.bfloat16, torch.float16, what=f"{what} out")
-    if tuple(out.shape) != (m, n) or (n > 1 and out.stride(1) != 1) or (m > 1 and out.stride(0) < n):
-        raise ValueError(f"{what}: out must be [{m}, {n}] with unit column stride and rows that do not overlap, got "
-                         f"{tuple(out.shape)} with strides {out.stride()}")
-    return out
-
-
-def _ld(t: torch.Tensor) -> int:
-    """The row stride of a matrix; a single row may have any, and K (a multiple of 16) serves."""
-    return t.stride(-2) if t.shape[-2] > 1 else t.shape[-1]
+        out, ldy = torch.empty_strided((m, n), (n, 1), dtype=out_dtype, device=device), n
+    else:
+        _dt(out, torch.bfloat16, torch.float16, what=f"{what} out")
+        if tuple(out.shape) != (m, n) or (n > 1 and out.stride(1) != 1) or (m > 1 and out.stride(0) < n):
+            raise ValueError(f"{what}: out must be [{m}, {n}] with unit column stride and rows that do not overlap, got "
+                             f"{tuple(out.shape)} with strides {out.stride()}")
+        ldy = max(out.stride(0), n)
+    # a single row may have any stride; K (a multiple of 16) serves
+    if m <= 1:
+        lda = k
+    if n == 1:
+        w_strides = (*w_strides[:-2], k, 1)
+    return m, n, k, lda, w_strides, out, ldy
 
 
 def fp8_gemm_blocks(a: torch.Tensor, w: torch.Tensor, sa: torch.Tensor, sb: torch.Tensor,
@@ -580,13 +584,11 @@ def fp8_gemm_blocks(a: torch.Tensor, w: torch.Tensor, sa: torch.Tensor, sb: torc
     with sb [ceil(N/128), ceil(K/128)] fp32 (``quant_weight_blocks`` or a block-quantised checkpoint); scales of any
     strides.  K a multiple of 16, row strides of a and w too; any M and N.  fp32 sums, one rounding to out_dtype (bf16
     or f16); ``bias`` [N] bf16 is added before it."""
-    y = _block_product(a, w, sa, sb, bias, out_dtype, out, "fp8_gemm_blocks")
-    m, k = a.shape
-    n = w.shape[0]
-    bias = _bias(bias, n, "fp8_gemm_blocks")
-    _launch(a, "h3b_fp8_gemm_blocks", a.data_ptr(), _ld(a), w.data_ptr(), _ld(w), sa.data_ptr(), sa.stride(0),
-            sa.stride(1), sb.data_ptr(), sb.stride(0), sb.stride(1), _ptr(bias), y.data_ptr(), max(y.stride(0), n), m, n,
-            k, OUT_BF16 if y.dtype == torch.bfloat16 else OUT_F16)
+    m, n, k, lda, (ldw, _), y, ldy = _product_operands(a, w, sa, sb, (bias,), out_dtype, out, "fp8_gemm_blocks", 2)
+    if bias is not None:
+        bias = _bias(bias, n, "fp8_gemm_blocks")
+    _launch(a, "h3b_fp8_gemm_blocks", a.data_ptr(), lda, w.data_ptr(), ldw, sa.data_ptr(), *sa.stride(), sb.data_ptr(),
+            *sb.stride(), _ptr(bias), y.data_ptr(), ldy, m, n, k, OUT_BF16 if y.dtype == torch.bfloat16 else OUT_F16)
     return y
 
 
@@ -597,17 +599,18 @@ def fp8_gemm_grouped(a: torch.Tensor, w: torch.Tensor, sa: torch.Tensor, sb: tor
     device, non-decreasing within [0, T]; the host never reads them.  Groups may be empty.  Rows before offsets[0] and
     from offsets[E] on are not written (a fresh output is uninitialised there).  Bounds out of order or out of range
     skip their group and record H3B_EINVAL in the device status word (``device_status``)."""
-    if offsets.dtype not in (torch.int32, torch.int64):
+    wide = offsets.dtype == torch.int64
+    if not wide and offsets.dtype != torch.int32:
         raise TypeError(f"fp8_gemm_grouped: offsets {offsets.dtype}, expected int32 or int64")
-    y = _block_product(a, w, sa, sb, None, out_dtype, out, "fp8_gemm_grouped", offsets)
-    m, k = a.shape
-    e, n = w.shape[:2]
-    if tuple(offsets.shape) != (e + 1,) or e < 1:
+    m, n, k, lda, (w_exp, ldw, _), y, ldy = _product_operands(a, w, sa, sb, (offsets,), out_dtype, out,
+                                                              "fp8_gemm_grouped", 3)
+    e = w.shape[0]
+    if offsets.shape != (e + 1,) or e < 1:
         raise ValueError(f"fp8_gemm_grouped: offsets must be [{e + 1}] for {e} experts, got {tuple(offsets.shape)}")
-    offsets = offsets.contiguous()
-    _launch(a, "h3b_fp8_gemm_grouped", a.data_ptr(), _ld(a), w.data_ptr(), w.stride(0), _ld(w), sa.data_ptr(),
-            sa.stride(0), sa.stride(1), sb.data_ptr(), sb.stride(0), sb.stride(1), sb.stride(2), offsets.data_ptr(),
-            int(offsets.dtype == torch.int64), y.data_ptr(), max(y.stride(0), n), m, e, n, k,
+    if offsets.stride(0) != 1:
+        offsets = offsets.contiguous()
+    _launch(a, "h3b_fp8_gemm_grouped", a.data_ptr(), lda, w.data_ptr(), w_exp, ldw, sa.data_ptr(), *sa.stride(),
+            sb.data_ptr(), *sb.stride(), offsets.data_ptr(), wide, y.data_ptr(), ldy, m, e, n, k,
             OUT_BF16 if y.dtype == torch.bfloat16 else OUT_F16)
     return y
 
