@@ -3,9 +3,13 @@
 // those of the per-token quant, taken over a block:
 //   scale = max(amax / 448, 1/(448*512)),  q = e4m3_rn(clamp(h * (1 / scale), -448, 448))     (NaN propagates)
 //
-// Activations: 16 lanes hold a block as one 16-byte load each (8 bf16 values), reduce its abs-max with four shuffles
-// inside the half-warp and write 128 bytes of e4m3; no shared memory, no barrier.  Weights: a CTA of 256 threads holds
-// a 128 x 128 tile in registers (8 vectors per thread) and reduces it once.  Every value is read once and written once.
+// Activations: 16 lanes hold a block as one 16-byte load each (8 bf16 values), reduce its abs-max inside the half-warp and
+// write 128 bytes of e4m3; no shared memory, no barrier.  A warp takes the same block of eight consecutive rows: blocks
+// taken along a row instead, each with divisions and a 4-byte scale store of its own, ran at 4.9 TB/s (62,496 x 5,120:
+// 199 us), this at 6.4 (151 us; the copy rate is 6.46); two rows a half-warp instead of four: 5.5.  silu-mul, 31,248 x
+// 13,824: 361 us, 6.0 TB/s (blocks along a row 466; two rows 429; CTAs of 256 threads 385).  Weights: a CTA of 256 threads
+// holds a 128 x 128 tile in registers (8 vectors per thread) and reduces it once: 15,360 x 5,120 in 37 us, 6.35 TB/s (512
+// threads: 50 us).  Every value is read once and written once.
 #include "common.cuh"
 #include "quant.cuh"
 
@@ -62,60 +66,93 @@ __device__ __forceinline__ uint2 quant8f(const float (&y)[8], float inv) {
   return make_uint2(o[0], o[1]);
 }
 
-// the largest of the half-warp's 16 values, in each of its lanes
-__device__ __forceinline__ uint32_t half_warp_max(uint32_t v) {
-#pragma unroll
-  for (int o = 8; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
+// Maxima of U values over the 16 lanes of a half-warp in U + log2(16 / U) shuffles instead of 4 U: in each of the first
+// log2(U) steps a lane gives half of its values away and keeps the other half.  The lane is left with the maximum of
+// value owned<U>(lane).
+template <int U>
+__device__ __forceinline__ int owned(int hl) {
+  return U == 4 ? (hl >> 2 & 3) : (U == 2 ? hl >> 3 : 0);
+}
+template <int U>
+__device__ __forceinline__ uint32_t half_warp_max(const uint32_t (&v)[U], int hl) {
+  constexpr uint32_t ALL = 0xffffffffu;
+  uint32_t m;
+  if constexpr (U == 4) {
+    const bool hi = hl & 8;
+    uint32_t a = hi ? v[2] : v[0], b = hi ? v[3] : v[1];
+    a = max(a, __shfl_xor_sync(ALL, hi ? v[0] : v[2], 8));
+    b = max(b, __shfl_xor_sync(ALL, hi ? v[1] : v[3], 8));
+    const bool odd = hl & 4;
+    m = max(odd ? b : a, __shfl_xor_sync(ALL, odd ? a : b, 4));
+  } else if constexpr (U == 2) {
+    const bool hi = hl & 8;
+    m = max(hi ? v[1] : v[0], __shfl_xor_sync(ALL, hi ? v[0] : v[1], 8));
+    m = max(m, __shfl_xor_sync(ALL, m, 4));
+  } else {
+    static_assert(U == 1, "1, 2 or 4 values");
+    m = max(v[0], __shfl_xor_sync(ALL, v[0], 8));
+    m = max(m, __shfl_xor_sync(ALL, m, 4));
+  }
+  m = max(m, __shfl_xor_sync(ALL, m, 2));
+  return max(m, __shfl_xor_sync(ALL, m, 1));
 }
 
-// rows x [rows, K] (SILU: [rows, 2K], gate | up) -> q [rows, K], s[row * s_row + j * s_blk].  Block g = row * KB + j;
-// a CTA takes 16 * U consecutive blocks, its half-warps U each, 16 blocks apart, all loads in flight together.
+// rows x [rows, K] (SILU: [rows, 2K], gate | up) -> q [rows, K], s[row * s_row + j * s_blk].  A warp takes block j of 2U
+// consecutive rows, U per half-warp: their scales are then neighbours in the block-major scale tensor and leave in one
+// store, each division is made once per warp for 2U blocks, and the loads of a CTA's 4 warps run along the rows.
 template <bool VEC, bool SILU, int U>
-__global__ void __launch_bounds__(256) quant_blocks_kernel(const uint16_t* __restrict__ x, uint32_t total, uint32_t KB,
-                                                           int64_t K, int64_t stride_x, uint8_t* __restrict__ q,
-                                                           float* __restrict__ s, int64_t s_row, int64_t s_blk,
-                                                           int div_mode) {
+__global__ void __launch_bounds__(128) quant_blocks_kernel(const uint16_t* __restrict__ x, uint32_t rows, uint32_t units,
+                                                           uint32_t KB, int64_t K, int64_t stride_x,
+                                                           uint8_t* __restrict__ q, float* __restrict__ s, int64_t s_row,
+                                                           int64_t s_blk, int div_mode) {
   const int hl = threadIdx.x & 15;
-  const uint32_t g0 = blockIdx.x * (16u * U) + (threadIdx.x >> 4);
+  const uint32_t unit = blockIdx.x * 4u + (threadIdx.x >> 5);
+  if (unit >= units) return;  // the whole warp
+  const uint32_t group = unit / KB, j = unit - group * KB;
+  const uint32_t row0 = group * (2u * U) + (threadIdx.x & 16 ? U : 0u);
+  const int64_t c = static_cast<int64_t>(j) * BLK + hl * 8;
   uint4 v[U], w[U];
-  uint32_t row[U], j[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const uint32_t g = g0 + 16u * u;
-    row[u] = g / KB;
-    j[u] = g - row[u] * KB;
     v[u] = w[u] = make_uint4(0, 0, 0, 0);
-    if (g < total) {
-      const uint16_t* xr = x + row[u] * stride_x;
-      const int64_t c = static_cast<int64_t>(j[u]) * BLK + hl * 8;
+    if (row0 + u < rows) {
+      const uint16_t* xr = x + (row0 + u) * stride_x;
       v[u] = load8<VEC>(xr, c, K);
       if (SILU) w[u] = load8<VEC>(xr + K, c, K);
     }
   }
+  float y[SILU ? U : 1][8];
+  uint32_t amax[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    float y[8];
-    uint32_t amax;
-    if (SILU) {
+    if constexpr (SILU) {
       float f[8];
-      unpack8(v[u], y);
+      unpack8(v[u], y[u]);
       unpack8(w[u], f);
-      amax = 0;
+      amax[u] = 0;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        y[e] = silu_mul_f32(y[e], f[e]);
-        amax = max(amax, __float_as_uint(y[e]) & 0x7FFFFFFFu);  // NaN bits sort above every number
+        y[u][e] = silu_mul_f32(y[u][e], f[e]);
+        amax[u] = max(amax[u], __float_as_uint(y[u][e]) & 0x7FFFFFFFu);  // NaN bits sort above every number
       }
     } else {
-      amax = fold16(absmax8(v[u], 0)) << 16;
+      amax[u] = fold16(absmax8(v[u], 0)) << 16;
     }
-    const float scale = block_scale(half_warp_max(amax), div_mode);
-    const float inv = qdiv(1.0f, scale, div_mode);
-    if (g0 + 16u * u < total) {
-      store8<VEC>(q + row[u] * K, static_cast<int64_t>(j[u]) * BLK + hl * 8, K,
-                  SILU ? quant8f(y, inv) : quant8(v[u], inv));
-      if (hl == 0) s[row[u] * s_row + j[u] * s_blk] = scale;
+  }
+  const float scale = block_scale(half_warp_max<U>(amax, hl), div_mode);
+  const float inv = qdiv(1.0f, scale, div_mode);
+  const uint32_t mine = row0 + owned<U>(hl);
+  if (hl % (16 / U) == 0 && mine < rows) s[mine * s_row + j * s_blk] = scale;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const float inv_u = U == 1 ? inv : __shfl_sync(0xffffffffu, inv, (threadIdx.x & 16) + u * (16 / U));
+    if (row0 + u < rows) {
+      uint2 out;
+      if constexpr (SILU)
+        out = quant8f(y[u], inv_u);
+      else
+        out = quant8(v[u], inv_u);
+      store8<VEC>(q + (row0 + u) * K, c, K, out);
     }
   }
 }
@@ -127,6 +164,7 @@ __global__ void __launch_bounds__(256) quant_weight_blocks_kernel(const uint16_t
                                                                   uint32_t KB, uint8_t* __restrict__ q,
                                                                   float* __restrict__ s, int div_mode) {
   __shared__ uint32_t red[8];
+  __shared__ float inv_scale;
   const uint32_t tile = blockIdx.x;
   const uint32_t j = tile % KB, en = tile / KB, i = en % NB, e = en / NB;
   const int64_t c = static_cast<int64_t>(j) * BLK + (threadIdx.x & 15) * 8;
@@ -143,17 +181,21 @@ __global__ void __launch_bounds__(256) quant_weight_blocks_kernel(const uint16_t
   const uint32_t wmax = __reduce_max_sync(0xffffffffu, fold16(m2));
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = wmax;
   __syncthreads();
-  uint32_t amax = red[0];
+  if (threadIdx.x < 32) {  // the divisions in one warp: in all eight they took a tenth of the kernel
+    uint32_t amax = red[0];
 #pragma unroll
-  for (int k = 1; k < 8; ++k) amax = max(amax, red[k]);
-  const float scale = block_scale(amax << 16, div_mode);
-  const float inv = qdiv(1.0f, scale, div_mode);
+    for (int k = 1; k < 8; ++k) amax = max(amax, red[k]);
+    const float scale = block_scale(amax << 16, div_mode);
+    inv_scale = qdiv(1.0f, scale, div_mode);
+    if (threadIdx.x == 0) s[tile] = scale;
+  }
+  __syncthreads();
+  const float inv = inv_scale;
 #pragma unroll
   for (int u = 0; u < 8; ++u) {
     const int64_t r = r0 + 16 * u;
     if (r < N) store8<VEC>(q + (e * N + r) * K, c, K, quant8(v[u], inv));
   }
-  if (threadIdx.x == 0) s[tile] = scale;
 }
 
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
@@ -170,18 +212,20 @@ int quant_blocks(const char* what, const void* x, int64_t rows, int64_t K, int64
   if (stride_x < 0 || s_row < 0 || s_blk < 0) return fail(H3B_EINVAL, "%s: negative stride", what);
   const int64_t KB = (K + BLK - 1) / BLK;
   if (rows > ((1ll << 31) - 1) / KB) return fail(H3B_EUNSUPPORTED, "%s: 2^31 blocks or more", what);
-  const uint32_t total = static_cast<uint32_t>(rows * KB);
   const bool vec = K % 8 == 0 && stride_x % 8 == 0 && aligned(x, 16) && aligned(q, 8);
-  constexpr int U = SILU ? 2 : 4;
-  const unsigned grid = (total + 16 * U - 1) / (16 * U);
+  constexpr int U = 4;
+  const auto units = static_cast<uint32_t>((rows + 2 * U - 1) / (2 * U) * KB);
+  const unsigned grid = (units + 3) / 4;
   const auto* xx = static_cast<const uint16_t*>(x);
   auto* qq = static_cast<uint8_t*>(q);
   if (vec)
-    quant_blocks_kernel<true, SILU, U><<<grid, 256, 0, st>>>(xx, total, static_cast<uint32_t>(KB), K, stride_x, qq, s,
-                                                             s_row, s_blk, div_mode);
+    quant_blocks_kernel<true, SILU, U><<<grid, 128, 0, st>>>(xx, static_cast<uint32_t>(rows), units,
+                                                             static_cast<uint32_t>(KB), K, stride_x, qq, s, s_row, s_blk,
+                                                             div_mode);
   else
-    quant_blocks_kernel<false, SILU, U><<<grid, 256, 0, st>>>(xx, total, static_cast<uint32_t>(KB), K, stride_x, qq, s,
-                                                              s_row, s_blk, div_mode);
+    quant_blocks_kernel<false, SILU, U><<<grid, 128, 0, st>>>(xx, static_cast<uint32_t>(rows), units,
+                                                              static_cast<uint32_t>(KB), K, stride_x, qq, s, s_row, s_blk,
+                                                              div_mode);
   H3B_CHECK_LAUNCH(what);
   return H3B_OK;
 }

@@ -98,6 +98,20 @@ def test_quant_blocks_is_the_eager_formula(dev, m, k):
     assert float(((q.double() - v).abs() - half_step_e4m3(v) * (1 + 2.0 ** -18)).max()) <= 0
 
 
+def test_quant_blocks_every_bf16_maximum(dev):
+    """A block for each positive finite bf16 value as its maximum, and the whole tile of a weight likewise."""
+    top = torch.arange(1, 0x7F80, dtype=torch.int32, device=dev).to(torch.int16).view(BF16)
+    x = (torch.rand(top.numel(), 128, device=dev, generator=gen(1)) * 2 - 1) * top.float()[:, None]
+    x = torch.where(x.abs() > top.float()[:, None], 0.0, x).to(BF16)
+    x[:, 77] = -top
+    q, s = ops.quant_blocks(x)
+    rq, rs = quant_oracle(x)
+    assert torch.equal(s, rs) and torch.equal(codes(q), codes(rq))
+    tiles = x[:254].view(254, 1, 128).expand(254, 128, 128).contiguous()
+    q, s = ops.quant_weight_blocks(tiles)
+    assert torch.equal(s.view(-1), rs[:254, 0]) and torch.equal(codes(q[:, 5]), codes(rq[:254]))
+
+
 def test_quant_blocks_special_rows(dev):
     """Zero blocks take the smallest scale; a NaN or an infinity marks its own block only; subnormals and the largest
     value keep the formula."""
