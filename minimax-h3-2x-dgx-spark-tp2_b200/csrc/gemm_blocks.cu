@@ -124,14 +124,17 @@ __device__ __forceinline__ bool cluster_flag(uint32_t flag_smem) {
 // ---------------------------------------------------------------------------------------------------------------
 namespace wide {
 
-constexpr int BM = 128, BN = 256, STAGES = 6;
-constexpr int STAGE_BYTES = 2 * BM * BLK;           // this CTA's 128 rows of a and 128 rows of w, 128 bytes each
+constexpr int BM = 128, BN = 256;
+// a stage: 128 rows of a, and of w its half of the pair's 256 rows or (one CTA) all of them, 128 bytes each
+__host__ __device__ constexpr int stages(bool pair) { return pair ? 6 : 4; }
+__host__ __device__ constexpr int stage_bytes(bool pair) { return (BM + (pair ? BN / 2 : BN)) * BLK; }
+constexpr int RING_BYTES = stages(true) * stage_bytes(true);
+static_assert(RING_BYTES == stages(false) * stage_bytes(false), "the rings take the same room");
 constexpr int EPI_WARPS = 8, FIRST_EPI = 4, THREADS = 32 * (FIRST_EPI + EPI_WARPS);
-constexpr int MAX_SPLIT = 4, ROUND_COST = 14;        // a cluster of 8 CTAs at most
+constexpr int MAX_SPLIT = 8, ROUND_COST = 14;        // clusters of 8 CTAs at most: 4 parts for pairs
 constexpr int WARP_STAGING = 32 * 128;              // 32 rows x 64 columns of 16-bit output
-constexpr int SMEM = STAGES * STAGE_BYTES + 1024 + 1024 + EPI_WARPS * WARP_STAGING;
+constexpr int SMEM = RING_BYTES + 1024 + 1024 + EPI_WARPS * WARP_STAGING;
 static_assert(SMEM <= 232448, "shared memory");
-constexpr uint32_t IDESC = idesc_make(FMT_E4M3, FMT_E4M3, 0, 2 * BM, BN);
 // row blocks (256 rows) that share a column block's w tile in L2, as in the per-token product
 constexpr int GROUP_M = 16;
 
@@ -146,19 +149,21 @@ __device__ __forceinline__ void coords(int r, int blocks, int num_nb, int& mb, i
 }
 
 // SPLIT: clusters of p.split pairs take a tile each, every pair a part of K
-template <bool SPLIT>
+template <bool PAIR, bool SPLIT>
 __global__ void __launch_bounds__(THREADS, 1)
     kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
            const __grid_constant__ CUtensorMap tmY, const __grid_constant__ Params p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE_BYTES);
+  constexpr int STAGES = stages(PAIR), STAGE_BYTES = stage_bytes(PAIR), CTAS = PAIR ? 2 : 1;
+  constexpr uint32_t IDESC = idesc_make(FMT_E4M3, FMT_E4M3, 0, CTAS * BM, BN);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + RING_BYTES);
   // bars: full[STAGES], used[STAGES], tempty[2], done; then the TMEM address and the start flag.  used[s]: the MMAs of
   // the step in stage s are complete, which frees the stage for the producer and hands the step's accumulator to the
   // epilogue (one commit per step for both)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 3);
   uint32_t* start_flag = tmem_slot + 1;
-  uint8_t* staging = smem + STAGES * STAGE_BYTES + 1024;
+  uint8_t* staging = smem + RING_BYTES + 1024;
   const uint32_t smem0 = smem_u32(smem), bar0 = smem_u32(bars);
   auto full_bar = [&](int s) { return bar0 + 8u * s; };
   auto used_bar = [&](int s) { return bar0 + 8u * (STAGES + s); };
@@ -166,9 +171,10 @@ __global__ void __launch_bounds__(THREADS, 1)
   const uint32_t done_bar = bar0 + 8u * (2 * STAGES + 2);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = cluster_ctarank(), leader = SPLIT ? rank & ~1u : 0u;
-  const int crank = static_cast<int>(rank & 1u);  // 0: the pair's leader (issues the MMAs)
-  const int part = SPLIT ? static_cast<int>(rank >> 1) : 0;  // the pair's part of K: steps [kb0, kb1)
+  const uint32_t rank = PAIR || SPLIT ? cluster_ctarank() : 0u;
+  const int crank = PAIR ? static_cast<int>(rank & 1u) : 0;  // 0: the pair's leader (issues the MMAs)
+  const int part = SPLIT ? static_cast<int>(rank / CTAS) : 0;  // the part of K: steps [kb0, kb1)
+  const uint32_t leader = static_cast<uint32_t>(part * CTAS);
   const int kb0 = SPLIT ? static_cast<int>(static_cast<int64_t>(p.num_kb) * part / p.split) : 0;
   const int kb1 = SPLIT ? static_cast<int>(static_cast<int64_t>(p.num_kb) * (part + 1) / p.split) : p.num_kb;
   const uint16_t pair_mask = static_cast<uint16_t>(3u << leader);
@@ -177,7 +183,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       mbar_init(full_bar(s), 1);
       mbar_init(used_bar(s), 1);
     }
-    for (int b = 0; b < 2; ++b) mbar_init(tempty_bar(b), 2 * EPI_WARPS);  // every epilogue warp of both CTAs
+    for (int b = 0; b < 2; ++b) mbar_init(tempty_bar(b), CTAS * EPI_WARPS);  // every epilogue warp (of both CTAs)
     mbar_init(done_bar, 2);
     fence_mbar_init();
     *start_flag = status_bad(p.wc) ? 0u : 1u;
@@ -185,8 +191,13 @@ __global__ void __launch_bounds__(THREADS, 1)
     tma_prefetch_desc(&tmW);
   }
   if (warp == 1) {
-    tmem_alloc_pair(smem_u32(tmem_slot), 512);
-    tmem_relinquish_pair();
+    if constexpr (PAIR) {
+      tmem_alloc_pair(smem_u32(tmem_slot), 512);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(smem_u32(tmem_slot), 512);
+      tmem_relinquish();
+    }
   }
   tc_fence_before();
   cluster_sync();
@@ -194,7 +205,8 @@ __global__ void __launch_bounds__(THREADS, 1)
   const uint32_t tmem_base = *tmem_slot;
   const bool start = cluster_flag(smem_u32(start_flag));  // of the cluster's first CTA
   const int first_tile = static_cast<int>(cluster_id_x()), tile_step = static_cast<int>(cluster_count_x());
-  Walk<2 * BM> walk;
+  Walk<CTAS * BM> walk;
+  bool ok = true;  // no wait of this thread's role has given up
 
   if (warp < FIRST_EPI) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
@@ -204,11 +216,10 @@ __global__ void __launch_bounds__(THREADS, 1)
       int stage = 0;
       uint32_t phase = 0;
       uint32_t loaded = 0, last = 0;  // per stage: loaded at all, parity of its last load
-      bool ok = true;
       for (int64_t t = first_tile; ok && walk.find(p, t, p.num_nb); t += tile_step) {
         int mb, nb;
         coords(walk.r, walk.blocks, p.num_nb, mb, nb);
-        const int arow = static_cast<int>(walk.lo) + (2 * mb + crank) * BM;
+        const int arow = static_cast<int>(walk.lo) + (CTAS * mb + crank) * BM;
         const int wrow = nb * BN + crank * BM;
         if (lane == 0) {
           for (int kb = kb0; kb < kb1; ++kb) {
@@ -217,9 +228,15 @@ __global__ void __launch_bounds__(THREADS, 1)
               break;
             }
             const uint32_t sA = smem0 + stage * STAGE_BYTES;
-            if (crank == 0) mbar_arrive_expect_tx(full_bar(stage), 2 * STAGE_BYTES);
-            tma_load_2d_pair(sA, &tmA, lead_full0 + 8u * stage, kb * BLK, arow);
-            tma_load_3d_pair(sA + BM * BLK, &tmW, lead_full0 + 8u * stage, kb * BLK, wrow, walk.e);
+            if (crank == 0) mbar_arrive_expect_tx(full_bar(stage), CTAS * STAGE_BYTES);
+            if constexpr (PAIR) {
+              tma_load_2d_pair(sA, &tmA, lead_full0 + 8u * stage, kb * BLK, arow);
+              tma_load_3d_pair(sA + BM * BLK, &tmW, lead_full0 + 8u * stage, kb * BLK, wrow, walk.e);
+            } else {
+              tma_load_2d(sA, &tmA, full_bar(stage), kb * BLK, arow);
+              tma_load_3d(sA + BM * BLK, &tmW, full_bar(stage), kb * BLK, wrow, walk.e);
+              tma_load_3d(sA + 2 * BM * BLK, &tmW, full_bar(stage), kb * BLK, wrow + BM, walk.e);
+            }
             loaded |= 1u << stage;
             last = (last & ~(1u << stage)) | (phase << stage);
             if (++stage == STAGES) {
@@ -249,8 +266,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         // the tensor pipe is busy, and its waits and commits (~350 cycles a step) would leave the pipe idle.
         const int b = warp - 1;
         uint32_t it = 0;  // steps before this tile
-        bool ok = true;
-        for (int64_t t = first_tile; ok && walk.find(p, t, p.num_nb); t += tile_step, it += kb1 - kb0) {
+          for (int64_t t = first_tile; ok && walk.find(p, t, p.num_nb); t += tile_step, it += kb1 - kb0) {
           if (lane == 0) {
             for (uint32_t i = it + ((it ^ b) & 1u); i < it + (kb1 - kb0); i += 2) {
               const uint32_t round = i / STAGES, stage = i - round * STAGES;
@@ -263,15 +279,26 @@ __global__ void __launch_bounds__(THREADS, 1)
               const uint32_t sA = smem0 + stage * STAGE_BYTES;
               const uint64_t adesc = sdesc_sw128(sA, 16, 1024), bdesc = sdesc_sw128(sA + BM * BLK, 16, 1024);
 #pragma unroll
-              for (int kk = 0; kk < BLK / 32; ++kk)
-                umma_f8_ss_pair(tmem_base + static_cast<uint32_t>(b * BN), adesc + 2u * kk, bdesc + 2u * kk, IDESC, kk != 0);
-              umma_commit_pair_mc(used_bar(stage), pair_mask);
+              for (int kk = 0; kk < BLK / 32; ++kk) {
+                const uint32_t d = tmem_base + static_cast<uint32_t>(b * BN);
+                if constexpr (PAIR)
+                  umma_f8_ss_pair(d, adesc + 2u * kk, bdesc + 2u * kk, IDESC, kk != 0);
+                else
+                  umma_f8_ss(d, adesc + 2u * kk, bdesc + 2u * kk, IDESC, kk != 0);
+              }
+              if constexpr (PAIR)
+                umma_commit_pair_mc(used_bar(stage), pair_mask);
+              else
+                umma_commit(used_bar(stage));
             }
           }
           ok = __shfl_sync(0xffffffffu, ok, 0);
         }
         if (lane == 0) {  // every issued MMA completes before TMEM is released
-          umma_commit_pair(done_bar);
+          if constexpr (PAIR)
+            umma_commit_pair(done_bar);
+          else
+            umma_commit(done_bar);
           const uint64_t t0 = globaltimer();
           while (!mbar_try_wait(done_bar, 0) && globaltimer() - t0 < p.wc.timeout) {
           }
@@ -293,12 +320,12 @@ __global__ void __launch_bounds__(THREADS, 1)
       uint4* stg = reinterpret_cast<uint4*>(staging + (warp - FIRST_EPI) * WARP_STAGING);
       uint32_t it = 0, phase = 0;
       int stage = 0;
-      bool ok = true, have = false;
+      bool have = false;
       float acc[128];
       int mb = 0, nb = 0;
       for (int64_t t = first_tile; ok && walk.find(p, t, p.num_nb); t += tile_step) {
         coords(walk.r, walk.blocks, p.num_nb, mb, nb);
-        const int64_t m0 = walk.lo + (2 * mb + crank) * BM + sub * 32;  // the warp's first row
+        const int64_t m0 = walk.lo + (CTAS * mb + crank) * BM + sub * 32;  // the warp's first row
         const int64_t n0 = static_cast<int64_t>(nb) * BN + half * 128;  // and first column
         const bool row_ok = m0 + lane < walk.hi, col_ok = n0 < p.N;
         const float* sap = p.sa + (row_ok ? m0 + lane : walk.lo) * p.sa_row;
@@ -352,7 +379,12 @@ __global__ void __launch_bounds__(THREADS, 1)
           reg_fence(rb);
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive_cluster_relaxed(lead_tempty0 + 8u * b);
+          if (lane == 0) {
+            if constexpr (PAIR)
+              mbar_arrive_cluster_relaxed(lead_tempty0 + 8u * b);
+            else
+              mbar_arrive(tempty_bar(b));
+          }
           add(ra, 64);
           add(rb, 96);
         }
@@ -420,7 +452,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         __syncwarp();
         cluster_sync();
-        const int64_t m = walk.lo + (2 * mb + crank) * BM + sub * 32 + lane;
+        const int64_t m = walk.lo + (CTAS * mb + crank) * BM + sub * 32 + lane;
         if (have && m < walk.hi) {
           for (int g = part + half * p.split; g < BN / 16; g += 2 * p.split) {
             const int64_t n = static_cast<int64_t>(nb) * BN + 16 * g;
@@ -430,7 +462,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             for (int i = 0; i < 16; ++i) v[i] = 0.0f;
             for (int q = 0; q < p.split; ++q) {
               const uint32_t src = mapa_shared(smem0 + static_cast<uint32_t>((16 * g * BM + sub * 32 + lane) * 4),
-                                               static_cast<uint32_t>(2 * q + crank));
+                                               static_cast<uint32_t>(CTAS * q + crank));
 #pragma unroll
               for (int i = 0; i < 16; ++i) {
                 float x;
@@ -468,7 +500,12 @@ __global__ void __launch_bounds__(THREADS, 1)
   tc_fence_before();
   cluster_sync();  // neither CTA leaves (or frees the pair's TMEM) while the other may still signal it
   tc_fence_after();
-  if (warp == 1) tmem_dealloc_pair(tmem_base, 512);
+  if (warp == 1) {
+    if constexpr (PAIR)
+      tmem_dealloc_pair(tmem_base, 512);
+    else
+      tmem_dealloc(tmem_base, 512);
+  }
   if (walk.bad) record_status(p.wc, H3B_EINVAL);
 }
 
@@ -489,6 +526,8 @@ __host__ __device__ constexpr int stage_bytes(int nt) { return (BLK + nt) * BLK;
 // two CTAs per SM with a ring of 4 each: more than the ~45 KB in flight that an SM's share of the memory bandwidth needs,
 // and one CTA's start and end lie under the other's loads
 constexpr int CTAS_PER_SM = 2, STAGES = 4;
+// the epilogue follows the MMAs on the stages' barriers, whose phases it must not miss: MMAs run NBUF steps ahead at most
+static_assert(STAGES >= NBUF, "a stage's barrier would turn twice before the epilogue looks");
 // ring (reused for the sums that the cluster adds: NT x 128 fp32), barriers, two chunks of scales, alignment slack; at
 // least a third of an SM's shared memory, so that no more than two CTAs fit and their TMEM never exceeds 512 columns (a
 // CTA that waited for TMEM while its cluster waits for it could wait forever)
@@ -566,7 +605,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) kernel(const __grid_cons
         int stage = 0;
         uint32_t phase = 0;
         for (int kb = kb0; kb < kb1; ++kb) {
-          if (!mbar_wait(used_bar(stage), phase ^ 1u, p.wc)) break;
+          if (!mbar_wait_inline(used_bar(stage), phase ^ 1u, p.wc)) break;
           const uint32_t sW = smem0 + stage * STAGE_BYTES;
           mbar_arrive_expect_tx(full_bar(stage), STAGE_BYTES);
           tma_load_3d(sW, &tmW, full_bar(stage), kb * BLK, nb * BLK, walk.e);
@@ -591,7 +630,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) kernel(const __grid_cons
         uint32_t phase = 0, it = 0;
         for (int kb = kb0; kb < kb1; ++kb, ++it) {
           const int b = it % NBUF;
-          if (!mbar_wait(full_bar(stage), phase, p.wc) || !mbar_wait(tempty_bar(b), ((it / NBUF) & 1u) ^ 1u, p.wc)) break;
+          if (!mbar_wait_inline(full_bar(stage), phase, p.wc) || !mbar_wait_inline(tempty_bar(b), ((it / NBUF) & 1u) ^ 1u, p.wc)) break;
           tc_fence_after();
           const uint32_t sW = smem0 + stage * STAGE_BYTES;
           const uint64_t wdesc = sdesc_sw128(sW, 16, 1024), adesc = sdesc_sw128(sW + BLK * BLK, 16, 1024);
@@ -642,7 +681,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) kernel(const __grid_cons
 #pragma unroll 1
         for (int kb = c0; kb < c1; ++kb, ++it, s += NT) {
           const int b = it % NBUF;
-          ok = __all_sync(0xffffffffu, ok && mbar_wait(used_bar(stage), phase, p.wc));
+          ok = __all_sync(0xffffffffu, ok && mbar_wait_inline(used_bar(stage), phase, p.wc));
           if (!ok) break;
           if (++stage == STAGES) {
             stage = 0;
@@ -795,8 +834,8 @@ struct Fit {
 // `whole` / `parts`: the kernels for one part and for more.
 template <int MAX>
 int pick_split(Fit<MAX>& fits, const void* whole, const void* parts, int threads, int smem, int unit, int per_sm, int dev, int64_t tiles, int num_kb,
-               int round_cost, bool persistent, int* split, int* fit1) {
-  double best = 0;
+               int round_cost, bool persistent, int* split, int* fit1, double* best_cost) {
+  double& best = *best_cost;
   for (int s = 1; s <= MAX; ++s) {
     if (s > 1 && num_kb < 4 * s) break;  // four steps each at least
     int fit = 0;
@@ -818,43 +857,62 @@ int pick_split(Fit<MAX>& fits, const void* whole, const void* parts, int threads
   return H3B_OK;
 }
 
-int launch_wide(Params& p, const CUtensorMap& tmA, const CUtensorMap& tmW, int64_t tiles, int64_t expected, int dev,
-                cudaStream_t st) {
-  static Fit<wide::MAX_SPLIT> fits;
-  const void* whole = reinterpret_cast<const void*>(wide::kernel<false>);
-  const void* parts = reinterpret_cast<const void*>(wide::kernel<true>);
-  int fit = 0;
-  int rc = pick_split(fits, whole, parts, wide::THREADS, wide::SMEM, 2, 1, dev, expected, p.num_kb, wide::ROUND_COST, true, &p.split, &fit);
-  if (rc) return rc;
-  CUtensorMap tmY = tmA;  // a valid map where no TMA store is made
-  p.vec_out = al16(p.y) && p.ldy % 8 == 0;
-  if (p.vec_out) {
-    const uint64_t dims[2] = {static_cast<uint64_t>(p.N), static_cast<uint64_t>(p.T)};
-    const uint64_t strides[1] = {static_cast<uint64_t>(p.ldy) * 2};
-    const uint32_t box[2] = {64, 32};
-    rc = encode_tmap(&tmY, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, p.y, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
-    if (rc) return rc;
-    p.tma_out = 1;
+// a wide launch as planned: which kernels, over how many tiles, in how many parts of K
+template <bool PAIR>
+struct WidePlan {
+  int64_t tiles = 0;  // that there can be
+  int split = 1, fit = 0;
+  double cost = 0;    // in steps
+
+  static const void* whole() { return reinterpret_cast<const void*>(wide::kernel<PAIR, false>); }
+  static const void* parts() { return reinterpret_cast<const void*>(wide::kernel<PAIR, true>); }
+  // T rows in at most `active` groups of `experts`
+  int make(const Params& p, int64_t active, int dev) {
+    static Fit<PAIR ? wide::MAX_SPLIT / 2 : wide::MAX_SPLIT> fits;
+    constexpr int64_t ROWS = PAIR ? 2 * wide::BM : wide::BM;
+    tiles = (p.T + active * (ROWS - 1)) / ROWS * p.num_nb;
+    // to expect: T / ROWS and, where there are several groups, half a row block more for each
+    int64_t expected = p.experts == 1 ? tiles : (p.T + active * ROWS / 2) / ROWS * p.num_nb;
+    if (expected < 1) expected = 1;
+    return pick_split(fits, whole(), parts(), wide::THREADS, wide::SMEM, PAIR ? 2 : 1, 1, dev, expected, p.num_kb,
+                      wide::ROUND_COST, true, &split, &fit, &cost);
   }
-  // one part: as many pairs as run at once walk the tiles; more: a cluster for every tile that there can be
-  const int64_t clusters = p.split == 1 && tiles > fit ? fit : tiles;
-  void* args[] = {const_cast<CUtensorMap*>(&tmA), const_cast<CUtensorMap*>(&tmW), &tmY, &p};
-  return launch(p.split == 1 ? whole : parts, dim3(static_cast<unsigned>(2 * p.split * clusters), 1, 1), wide::THREADS, wide::SMEM, 2 * p.split, args,
-                st, nullptr);
-}
+  int go(Params& p, const CUtensorMap& tmA, const CUtensorMap& tmW, cudaStream_t st) {
+    p.split = split;
+    CUtensorMap tmY = tmA;  // a valid map where no TMA store is made
+    p.vec_out = al16(p.y) && p.ldy % 8 == 0;
+    if (p.vec_out) {
+      const uint64_t dims[2] = {static_cast<uint64_t>(p.N), static_cast<uint64_t>(p.T)};
+      const uint64_t strides[1] = {static_cast<uint64_t>(p.ldy) * 2};
+      const uint32_t box[2] = {64, 32};
+      const int rc = encode_tmap(&tmY, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, p.y, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+      if (rc) return rc;
+      p.tma_out = 1;
+    }
+    // one part: as many CTAs (pairs) as run at once walk the tiles; more: a cluster for every tile that there can be
+    const int64_t clusters = split == 1 && tiles > fit ? fit : tiles;
+    const int cluster = (PAIR ? 2 : 1) * split;
+    void* args[] = {const_cast<CUtensorMap*>(&tmA), const_cast<CUtensorMap*>(&tmW), &tmY, &p};
+    return launch(split == 1 ? whole() : parts(), dim3(static_cast<unsigned>(cluster * clusters), 1, 1), wide::THREADS,
+                  wide::SMEM, cluster, args, st, nullptr);
+  }
+};
 
 template <int NT>
 int launch_narrow(Params& p, const CUtensorMap& tmA, const CUtensorMap& tmW, int64_t token_tiles, int dev, cudaStream_t st) {
   static Fit<narrow::MAX_SPLIT> fits;
   const void* kernel = reinterpret_cast<const void*>(narrow::kernel<NT>);
   int fit = 0;
+  double cost = 0;
   const int rc = pick_split(fits, kernel, kernel, narrow::THREADS, narrow::smem(NT), 1, narrow::CTAS_PER_SM, dev, token_tiles * p.num_nb, p.num_kb,
-                            narrow::ROUND_COST, false, &p.split, &fit);
+                            narrow::ROUND_COST, false, &p.split, &fit, &cost);
   if (rc) return rc;
   void* args[] = {const_cast<CUtensorMap*>(&tmA), const_cast<CUtensorMap*>(&tmW), &p};
   return launch(kernel, dim3(static_cast<unsigned>(p.num_nb * p.split), static_cast<unsigned>(token_tiles), 1),
                 narrow::THREADS, narrow::smem(NT), p.split, args, st, nullptr);
 }
+
+constexpr double SINGLE_STEP = 1.05;  // a step of single CTAs against one of pairs
 
 struct Operands {
   const void* a;
@@ -924,13 +982,18 @@ int gemm_blocks(const char* what, const Operands& o, cudaStream_t st) {
   const int64_t mean = (o.T + o.E - 1) / o.E;
   if (mean > 64) {
     p.num_nb = static_cast<int>((o.N + wide::BN - 1) / wide::BN);
-    const int64_t tiles = (o.T + active * (2 * wide::BM - 1)) / (2 * wide::BM) * p.num_nb;
-    if (tiles > most / (2 * wide::MAX_SPLIT)) return fail(H3B_EUNSUPPORTED, "%s: 2^31 tiles or more", what);
+    if (active > most / p.num_nb || o.T / wide::BM + active > most / (2 * wide::MAX_SPLIT) / p.num_nb)
+      return fail(H3B_EUNSUPPORTED, "%s: 2^31 tiles or more", what);
     rc = load_map(&tmA, o.a, o.K, o.T, o.lda, wide::BM);
     if (rc) return rc;
-    // the tiles to expect: rows / 256 and, where there are several groups, half a row block more for each
-    const int64_t expected = o.E == 1 ? tiles : (o.T + active * wide::BM) / (2 * wide::BM) * p.num_nb;
-    return launch_wide(p, tmA, tmW, tiles, expected < 1 ? 1 : expected, dev, st);
+    // CTA pairs read less (32 KB a step and SM instead of 48) and win by about 8 % where both take as many rounds; single
+    // CTAs, with tiles of half the rows, fit small and ragged work better: 777 x 5,120 x 13,824 in 64 us against 113
+    WidePlan<true> pairs;
+    WidePlan<false> singles;
+    rc = pairs.make(p, active, dev);
+    if (!rc) rc = singles.make(p, active, dev);
+    if (rc) return rc;
+    return pairs.cost <= SINGLE_STEP * singles.cost ? pairs.go(p, tmA, tmW, st) : singles.go(p, tmA, tmW, st);
   }
   const int nt = mean <= 16 ? 16 : (mean <= 32 ? 32 : 64);
   p.num_nb = static_cast<int>((o.N + BLK - 1) / BLK);
