@@ -105,6 +105,8 @@ __global__ void __launch_bounds__(128) quant_blocks_kernel(const uint16_t* __res
                                                            uint32_t KB, int64_t K, int64_t stride_x,
                                                            uint8_t* __restrict__ q, float* __restrict__ s, int64_t s_row,
                                                            int64_t s_blk, int div_mode) {
+  pdl_wait();
+  pdl_launch();
   const int hl = threadIdx.x & 15;
   const uint32_t unit = blockIdx.x * 4u + (threadIdx.x >> 5);
   if (unit >= units) return;  // the whole warp
@@ -165,6 +167,8 @@ __global__ void __launch_bounds__(256) quant_weight_blocks_kernel(const uint16_t
                                                                   float* __restrict__ s, int div_mode) {
   __shared__ uint32_t red[8];
   __shared__ float inv_scale;
+  pdl_wait();
+  pdl_launch();
   const uint32_t tile = blockIdx.x;
   const uint32_t j = tile % KB, en = tile / KB, i = en % NB, e = en / NB;
   const int64_t c = static_cast<int64_t>(j) * BLK + (threadIdx.x & 15) * 8;
@@ -202,6 +206,21 @@ bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p
 
 int bad_mode(int div_mode) { return div_mode != H3B_DIV_IEEE && div_mode != H3B_DIV_FULL; }
 
+template <typename... P, typename... A>
+int launch(const char* what, void (*kernel)(P...), unsigned grid, unsigned threads, cudaStream_t st, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid, 1, 1);
+  cfg.blockDim = dim3(threads, 1, 1);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+  return e == cudaSuccess ? H3B_OK : cuda_fail(e, what);
+}
+
 template <bool SILU>
 int quant_blocks(const char* what, const void* x, int64_t rows, int64_t K, int64_t stride_x, void* q, float* s,
                  int64_t s_row, int64_t s_blk, int32_t div_mode, cudaStream_t st) {
@@ -218,16 +237,9 @@ int quant_blocks(const char* what, const void* x, int64_t rows, int64_t K, int64
   const unsigned grid = (units + 3) / 4;
   const auto* xx = static_cast<const uint16_t*>(x);
   auto* qq = static_cast<uint8_t*>(q);
-  if (vec)
-    quant_blocks_kernel<true, SILU, U><<<grid, 128, 0, st>>>(xx, static_cast<uint32_t>(rows), units,
-                                                             static_cast<uint32_t>(KB), K, stride_x, qq, s, s_row, s_blk,
-                                                             div_mode);
-  else
-    quant_blocks_kernel<false, SILU, U><<<grid, 128, 0, st>>>(xx, static_cast<uint32_t>(rows), units,
-                                                              static_cast<uint32_t>(KB), K, stride_x, qq, s, s_row, s_blk,
-                                                              div_mode);
-  H3B_CHECK_LAUNCH(what);
-  return H3B_OK;
+  return launch(what, vec ? quant_blocks_kernel<true, SILU, U> : quant_blocks_kernel<false, SILU, U>, grid, 128, st, xx,
+                static_cast<uint32_t>(rows), units, static_cast<uint32_t>(KB), K, stride_x, qq, s, s_row, s_blk,
+                static_cast<int>(div_mode));
 }
 
 }  // namespace
@@ -265,12 +277,7 @@ extern "C" int h3b_quant_weight_blocks_e4m3(const void* w, int64_t experts, int6
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const auto* ww = static_cast<const uint16_t*>(w);
   auto* qq = static_cast<uint8_t*>(q);
-  if (vec)
-    quant_weight_blocks_kernel<true><<<grid, 256, 0, st>>>(ww, n, k, stride_e, stride_n, static_cast<uint32_t>(NB),
-                                                           static_cast<uint32_t>(KB), qq, scale, div_mode);
-  else
-    quant_weight_blocks_kernel<false><<<grid, 256, 0, st>>>(ww, n, k, stride_e, stride_n, static_cast<uint32_t>(NB),
-                                                            static_cast<uint32_t>(KB), qq, scale, div_mode);
-  H3B_CHECK_LAUNCH("quant_weight_blocks launch");
-  return H3B_OK;
+  return launch("quant_weight_blocks", vec ? quant_weight_blocks_kernel<true> : quant_weight_blocks_kernel<false>, grid,
+                256, st, ww, n, k, stride_e, stride_n, static_cast<uint32_t>(NB), static_cast<uint32_t>(KB), qq, scale,
+                static_cast<int>(div_mode));
 }

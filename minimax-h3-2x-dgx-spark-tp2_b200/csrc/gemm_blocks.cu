@@ -186,7 +186,6 @@ __global__ void __launch_bounds__(THREADS, 1)
     for (int b = 0; b < 2; ++b) mbar_init(tempty_bar(b), CTAS * EPI_WARPS);  // every epilogue warp (of both CTAs)
     mbar_init(done_bar, 2);
     fence_mbar_init();
-    *start_flag = status_bad(p.wc) ? 0u : 1u;
     tma_prefetch_desc(&tmA);
     tma_prefetch_desc(&tmW);
   }
@@ -199,9 +198,12 @@ __global__ void __launch_bounds__(THREADS, 1)
       tmem_relinquish();
     }
   }
+  pdl_wait();
+  if (threadIdx.x == 0) *start_flag = status_bad(p.wc) ? 0u : 1u;
   tc_fence_before();
   cluster_sync();
   tc_fence_after();
+  pdl_launch();
   const uint32_t tmem_base = *tmem_slot;
   const bool start = cluster_flag(smem_u32(start_flag));  // of the cluster's first CTA
   const int first_tile = static_cast<int>(cluster_id_x()), tile_step = static_cast<int>(cluster_count_x());
@@ -565,6 +567,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) kernel(const __grid_cons
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int split = p.split;  // CTAs of the cluster: they share blockIdx.x / split
   const int crank = static_cast<int>(blockIdx.x) % split, nb = static_cast<int>(blockIdx.x) / split;
+  if (p.offsets != nullptr) pdl_wait();  // the bounds are the first thing read
   Walk<NT> walk;
   const bool found = walk.find(p, blockIdx.y, 1);  // the same for every CTA of the cluster
   if (!found) {
@@ -583,15 +586,19 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) kernel(const __grid_cons
     for (int b = 0; b < NBUF; ++b) mbar_init(tempty_bar(b), EPI_WARPS);
     mbar_init(done_bar, 1);
     fence_mbar_init();
-    *start_flag = status_bad(p.wc) ? 0u : 1u;
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmW);
   }
   if (warp == 1) {
     tmem_alloc(smem_u32(tmem_slot), TMEM_COLS);
     tmem_relinquish();
   }
+  pdl_wait();
+  if (threadIdx.x == 0) *start_flag = status_bad(p.wc) ? 0u : 1u;
   tc_fence_before();
   cluster_sync();
   tc_fence_after();
+  pdl_launch();
   const uint32_t tmem_base = *tmem_slot;
   const bool start = cluster_flag(smem_u32(start_flag));
   float acc[MINE];
@@ -793,13 +800,15 @@ int launch(const void* kernel, dim3 grid, int threads, int smem, int cluster, vo
   cfg.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
   cfg.dynamicSmemBytes = static_cast<size_t>(smem);
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = static_cast<unsigned>(cluster);
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = fit != nullptr ? 1 : 2;
   // with `fit`: no launch, but how many such clusters run at once
   const cudaError_t e = fit != nullptr ? cudaOccupancyMaxActiveClusters(fit, kernel, &cfg) : cudaLaunchKernelExC(&cfg, kernel, args);
   if (e != cudaSuccess) return cuda_fail(e, fit != nullptr ? "fp8_gemm_blocks: cluster occupancy" : "fp8_gemm_blocks launch");

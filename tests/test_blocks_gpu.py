@@ -478,6 +478,67 @@ def test_captured_with_new_inputs_and_sizes(dev):
         assert torch.equal(y, ffn(x, *packed, off)[-1])
 
 
+def test_captured_behind_copies_and_a_joined_stream(dev):
+    """The launches' programmatic edges where the node before is a copy or a memset, or there are two of them."""
+    packed = ffn_weights(512, 384)
+    src = torch.randn(40, 512, device=dev, generator=gen(1)).to(BF16)
+    x, y2 = torch.empty_like(src), torch.empty(40, 512, dtype=BF16, device=dev)
+    a, w, sa, sb = operands(40, 512, 640)
+    ffn(src, *packed)
+    torch.cuda.synchronize()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph):
+        x.zero_()
+        x.copy_(src)
+        y = ffn(x, *packed)[-1]
+        here = torch.cuda.current_stream()
+        side.wait_stream(here)
+        with torch.cuda.stream(side):
+            ops.fp8_gemm_blocks(a, w, sa, sb, out=y2)
+            q2, s2 = ops.quant_blocks(y2)
+        q1, s1 = ops.quant_blocks(y)
+        here.wait_stream(side)
+        z = ops.fp8_gemm_blocks(q1, w[:, :512].contiguous(), s1, sb[:, :4].contiguous())
+        z2 = ops.fp8_gemm_blocks(q2, w[:, :512].contiguous(), s2, sb[:, :4].contiguous())
+        x.zero_()
+    for seed in (5, 6):
+        src.copy_(torch.randn(40, 512, device=dev, generator=gen(seed)).to(BF16))
+        graph.replay()
+        want = ffn(src, *packed)[-1]
+        assert torch.equal(y, want)
+        assert torch.equal(z, ops.fp8_gemm_blocks(*_as_product(want, w, sb)))
+        assert torch.equal(z2, ops.fp8_gemm_blocks(*_as_product(ops.fp8_gemm_blocks(a, w, sa, sb), w, sb)))
+        assert bool((x == 0).all())
+
+
+def _as_product(y, w, sb):
+    q, s = ops.quant_blocks(y)
+    return q, w[:, :512].contiguous(), s, sb[:, :4].contiguous()
+
+
+def test_back_to_back_launches_see_each_other(dev):
+    """Every kernel may start before the one ahead of it on the stream ends: chains through the same buffers, with other
+    kernels in between, give what launches one at a time give."""
+    packed = ffn_weights(512, 384)
+    xs = [torch.randn(m, 512, device=dev, generator=gen(m)).to(BF16) for m in (1, 40, 300, 17, 2000, 3)]
+    want = []
+    for x in xs:
+        stages = ffn(x, *packed)
+        torch.cuda.synchronize()
+        want.append(ffn(stages[-1] * 0.5, *packed)[-1].clone())
+        torch.cuda.synchronize()
+    for _ in range(20):
+        got = []
+        for x in xs:
+            y = ffn(x, *packed)[-1]
+            y.mul_(0.5)
+            y = ffn(y, *packed)[-1]
+            got.append(y.clone())
+            y.fill_(float("nan"))          # the next call's buffers may be this one's
+        for g, w in zip(got, want):
+            assert torch.equal(g, w)
+
+
 def test_two_streams_at_once(dev):
     a, w, sa, sb = operands(40, 1024, 2048, seed=3)
     b, v, sc, sd = operands(500, 1024, 2048, seed=4)
