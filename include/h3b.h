@@ -233,7 +233,8 @@ H3B_API int h3b_fp8_gemm_blocks(const void* a, int64_t lda, const void* w, int64
  * a multiple of 16) and sb[e] (expert stride sb_expert).  offsets: experts + 1 device integers (offsets_i64 != 0: int64,
  * else int32), non-decreasing, within [0, rows]; groups may be empty, and rows before the first or behind the last
  * bound are neither used nor written.  A group whose bounds break this is skipped and H3B_EINVAL recorded in the device
- * status word.  The sizes are read on the device only. */
+ * status word; rows that two other groups then claim hold the product of either or of neither.  The sizes are read on the
+ * device only. */
 H3B_API int h3b_fp8_gemm_grouped(const void* a, int64_t lda, const void* w, int64_t w_expert, int64_t ldw,
                                  const float* sa, int64_t sa_row, int64_t sa_block, const float* sb, int64_t sb_expert,
                                  int64_t sb_row, int64_t sb_block, const void* offsets, int32_t offsets_i64, void* y,

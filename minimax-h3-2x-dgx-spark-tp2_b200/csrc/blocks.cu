@@ -6,9 +6,9 @@
 // Activations: 16 lanes hold a block as one 16-byte load each (8 bf16 values), reduce its abs-max inside the half-warp and
 // write 128 bytes of e4m3; no shared memory, no barrier.  A warp takes the same block of eight consecutive rows: blocks
 // taken along a row instead, each with divisions and a 4-byte scale store of its own, ran at 4.9 TB/s (62,496 x 5,120:
-// 199 us), this at 6.4 (151 us; the copy rate is 6.46); two rows a half-warp instead of four: 5.5.  silu-mul, 31,248 x
+// 199 us), this at 6.4 (151 us; the copy rate is 6.46).  silu-mul, 31,248 x
 // 13,824: 361 us, 6.0 TB/s (blocks along a row 466; two rows 429; CTAs of 256 threads 385).  Weights: a CTA of 256 threads
-// holds a 128 x 128 tile in registers (8 vectors per thread) and reduces it once: 15,360 x 5,120 in 37 us, 6.35 TB/s (512
+// holds a 128 x 128 tile in registers (8 vectors per thread) and reduces it once: 15,360 x 5,120 in 36 us, 6.5 TB/s (512
 // threads: 50 us).  Every value is read once and written once.
 #include "common.cuh"
 #include "quant.cuh"
@@ -66,33 +66,18 @@ __device__ __forceinline__ uint2 quant8f(const float (&y)[8], float inv) {
   return make_uint2(o[0], o[1]);
 }
 
-// Maxima of U values over the 16 lanes of a half-warp in U + log2(16 / U) shuffles instead of 4 U: in each of the first
-// log2(U) steps a lane gives half of its values away and keeps the other half.  The lane is left with the maximum of
-// value owned<U>(lane).
-template <int U>
-__device__ __forceinline__ int owned(int hl) {
-  return U == 4 ? (hl >> 2 & 3) : (U == 2 ? hl >> 3 : 0);
-}
-template <int U>
+constexpr int U = 4;  // rows of a half-warp (two: 5.5 TB/s where four make 6.4)
+
+// Maxima of four values over the 16 lanes of a half-warp in 5 shuffles instead of 16: in each of the first two steps a lane
+// gives half of its values away and keeps the other half.  Lane hl is left with the maximum of value hl / 4.
 __device__ __forceinline__ uint32_t half_warp_max(const uint32_t (&v)[U], int hl) {
+  static_assert(U == 4, "two halving steps");
   constexpr uint32_t ALL = 0xffffffffu;
-  uint32_t m;
-  if constexpr (U == 4) {
-    const bool hi = hl & 8;
-    uint32_t a = hi ? v[2] : v[0], b = hi ? v[3] : v[1];
-    a = max(a, __shfl_xor_sync(ALL, hi ? v[0] : v[2], 8));
-    b = max(b, __shfl_xor_sync(ALL, hi ? v[1] : v[3], 8));
-    const bool odd = hl & 4;
-    m = max(odd ? b : a, __shfl_xor_sync(ALL, odd ? a : b, 4));
-  } else if constexpr (U == 2) {
-    const bool hi = hl & 8;
-    m = max(hi ? v[1] : v[0], __shfl_xor_sync(ALL, hi ? v[0] : v[1], 8));
-    m = max(m, __shfl_xor_sync(ALL, m, 4));
-  } else {
-    static_assert(U == 1, "1, 2 or 4 values");
-    m = max(v[0], __shfl_xor_sync(ALL, v[0], 8));
-    m = max(m, __shfl_xor_sync(ALL, m, 4));
-  }
+  const bool hi = hl & 8, odd = hl & 4;
+  uint32_t a = hi ? v[2] : v[0], b = hi ? v[3] : v[1];
+  a = max(a, __shfl_xor_sync(ALL, hi ? v[0] : v[2], 8));
+  b = max(b, __shfl_xor_sync(ALL, hi ? v[1] : v[3], 8));
+  uint32_t m = max(odd ? b : a, __shfl_xor_sync(ALL, odd ? a : b, 4));
   m = max(m, __shfl_xor_sync(ALL, m, 2));
   return max(m, __shfl_xor_sync(ALL, m, 1));
 }
@@ -100,7 +85,7 @@ __device__ __forceinline__ uint32_t half_warp_max(const uint32_t (&v)[U], int hl
 // rows x [rows, K] (SILU: [rows, 2K], gate | up) -> q [rows, K], s[row * s_row + j * s_blk].  A warp takes block j of 2U
 // consecutive rows, U per half-warp: their scales are then neighbours in the block-major scale tensor and leave in one
 // store, each division is made once per warp for 2U blocks, and the loads of a CTA's 4 warps run along the rows.
-template <bool VEC, bool SILU, int U>
+template <bool VEC, bool SILU>
 __global__ void __launch_bounds__(128) quant_blocks_kernel(const uint16_t* __restrict__ x, uint32_t rows, uint32_t units,
                                                            uint32_t KB, int64_t K, int64_t stride_x,
                                                            uint8_t* __restrict__ q, float* __restrict__ s, int64_t s_row,
@@ -141,13 +126,13 @@ __global__ void __launch_bounds__(128) quant_blocks_kernel(const uint16_t* __res
       amax[u] = fold16(absmax8(v[u], 0)) << 16;
     }
   }
-  const float scale = block_scale(half_warp_max<U>(amax, hl), div_mode);
+  const float scale = block_scale(half_warp_max(amax, hl), div_mode);
   const float inv = qdiv(1.0f, scale, div_mode);
-  const uint32_t mine = row0 + owned<U>(hl);
-  if (hl % (16 / U) == 0 && mine < rows) s[mine * s_row + j * s_blk] = scale;
+  const uint32_t mine = row0 + hl / 4;
+  if (hl % 4 == 0 && mine < rows) s[mine * s_row + j * s_blk] = scale;
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const float inv_u = U == 1 ? inv : __shfl_sync(0xffffffffu, inv, (threadIdx.x & 16) + u * (16 / U));
+    const float inv_u = __shfl_sync(0xffffffffu, inv, (threadIdx.x & 16) + u * 4);
     if (row0 + u < rows) {
       uint2 out;
       if constexpr (SILU)
@@ -166,7 +151,7 @@ __global__ void __launch_bounds__(256) quant_weight_blocks_kernel(const uint16_t
                                                                   uint32_t KB, uint8_t* __restrict__ q,
                                                                   float* __restrict__ s, int div_mode) {
   __shared__ uint32_t red[8];
-  __shared__ float inv_scale;
+  __shared__ float tile_scale[2];  // and its inverse
   pdl_wait();
   pdl_launch();
   const uint32_t tile = blockIdx.x;
@@ -185,16 +170,17 @@ __global__ void __launch_bounds__(256) quant_weight_blocks_kernel(const uint16_t
   const uint32_t wmax = __reduce_max_sync(0xffffffffu, fold16(m2));
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = wmax;
   __syncthreads();
-  if (threadIdx.x < 32) {  // the divisions in one warp: in all eight they took a tenth of the kernel
-    uint32_t amax = red[0];
+  uint32_t amax = red[0];
 #pragma unroll
-    for (int k = 1; k < 8; ++k) amax = max(amax, red[k]);
+  for (int k = 1; k < 8; ++k) amax = max(amax, red[k]);
+  if (threadIdx.x < 32) {  // the divisions in one warp: in all eight they took a tenth of the kernel
     const float scale = block_scale(amax << 16, div_mode);
-    inv_scale = qdiv(1.0f, scale, div_mode);
-    if (threadIdx.x == 0) s[tile] = scale;
+    tile_scale[0] = scale;
+    tile_scale[1] = qdiv(1.0f, scale, div_mode);
   }
   __syncthreads();
-  const float inv = inv_scale;
+  const float inv = tile_scale[1];
+  if (threadIdx.x == 0) s[tile] = tile_scale[0];  // behind the barrier: ahead of it the others waited for it, 39.4 us for 36
 #pragma unroll
   for (int u = 0; u < 8; ++u) {
     const int64_t r = r0 + 16 * u;
@@ -232,12 +218,11 @@ int quant_blocks(const char* what, const void* x, int64_t rows, int64_t K, int64
   const int64_t KB = (K + BLK - 1) / BLK;
   if (rows > ((1ll << 31) - 1) / KB) return fail(H3B_EUNSUPPORTED, "%s: 2^31 blocks or more", what);
   const bool vec = K % 8 == 0 && stride_x % 8 == 0 && aligned(x, 16) && aligned(q, 8);
-  constexpr int U = 4;
   const auto units = static_cast<uint32_t>((rows + 2 * U - 1) / (2 * U) * KB);
   const unsigned grid = (units + 3) / 4;
   const auto* xx = static_cast<const uint16_t*>(x);
   auto* qq = static_cast<uint8_t*>(q);
-  return launch(what, vec ? quant_blocks_kernel<true, SILU, U> : quant_blocks_kernel<false, SILU, U>, grid, 128, st, xx,
+  return launch(what, vec ? quant_blocks_kernel<true, SILU> : quant_blocks_kernel<false, SILU>, grid, 128, st, xx,
                 static_cast<uint32_t>(rows), units, static_cast<uint32_t>(KB), K, stride_x, qq, s, s_row, s_blk,
                 static_cast<int>(div_mode));
 }

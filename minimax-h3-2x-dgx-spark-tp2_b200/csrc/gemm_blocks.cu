@@ -42,7 +42,7 @@ struct Params {
   int64_t ldy;
   int out_f16;
   int tma_out;        // wide: whole slices leave through TMA stores
-  int vec_out;        // y rows are 16-byte granular
+  int vec_out;        // y rows are 16-byte granular (narrow: 8-byte)
   WaitCtl wc;
 };
 
@@ -202,11 +202,13 @@ __global__ void __launch_bounds__(THREADS, 1)
   if (threadIdx.x == 0) *start_flag = status_bad(p.wc) ? 0u : 1u;
   tc_fence_before();
   cluster_sync();
-  tc_fence_after();
-  pdl_launch();
+  tc_fence_after();  // no pdl_launch in this form: the next kernel starting as CTAs leave cost an FFN chain of 256 rows 3 of 89 us
   const uint32_t tmem_base = *tmem_slot;
   const bool start = cluster_flag(smem_u32(start_flag));  // of the cluster's first CTA
   const int first_tile = static_cast<int>(cluster_id_x()), tile_step = static_cast<int>(cluster_count_x());
+  // parts of K: a cluster takes one tile.  Bounds that overlap make more tiles than the launch counted on: those are left
+  // out (the last find only looks for the bad bounds that there must be)
+  auto next_tile = [&](int64_t t) { return SPLIT ? INT64_MAX : t + tile_step; };
   Walk<CTAS * BM> walk;
   bool ok = true;  // no wait of this thread's role has given up
 
@@ -218,7 +220,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       int stage = 0;
       uint32_t phase = 0;
       uint32_t loaded = 0, last = 0;  // per stage: loaded at all, parity of its last load
-      for (int64_t t = first_tile; ok && walk.find(p, t, p.num_nb); t += tile_step) {
+      for (int64_t t = first_tile; ok && walk.find(p, t, p.num_nb); t = next_tile(t)) {
         int mb, nb;
         coords(walk.r, walk.blocks, p.num_nb, mb, nb);
         const int arow = static_cast<int>(walk.lo) + (CTAS * mb + crank) * BM;
@@ -268,7 +270,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         // the tensor pipe is busy, and its waits and commits (~350 cycles a step) would leave the pipe idle.
         const int b = warp - 1;
         uint32_t it = 0;  // steps before this tile
-          for (int64_t t = first_tile; ok && walk.find(p, t, p.num_nb); t += tile_step, it += kb1 - kb0) {
+        for (int64_t t = first_tile; ok && walk.find(p, t, p.num_nb); t = next_tile(t), it += kb1 - kb0) {
           if (lane == 0) {
             for (uint32_t i = it + ((it ^ b) & 1u); i < it + (kb1 - kb0); i += 2) {
               const uint32_t round = i / STAGES, stage = i - round * STAGES;
@@ -325,7 +327,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       bool have = false;
       float acc[128];
       int mb = 0, nb = 0;
-      for (int64_t t = first_tile; ok && walk.find(p, t, p.num_nb); t += tile_step) {
+      for (int64_t t = first_tile; ok && walk.find(p, t, p.num_nb); t = next_tile(t)) {
         coords(walk.r, walk.blocks, p.num_nb, mb, nb);
         const int64_t m0 = walk.lo + (CTAS * mb + crank) * BM + sub * 32;  // the warp's first row
         const int64_t n0 = static_cast<int64_t>(nb) * BN + half * 128;  // and first column
@@ -631,6 +633,13 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) kernel(const __grid_cons
           }
         }
       }
+      __syncwarp();
+      // bad bounds behind the last tile: one CTA looks at all of them
+      if (blockIdx.x == 0 && blockIdx.y == 0) {
+        Walk<NT> rest;
+        rest.find(p, INT64_MAX, 1);
+        walk.bad |= rest.bad;
+      }
     } else if (warp == 1) {
       if (lane == 0) {
         int stage = 0;
@@ -748,20 +757,39 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) kernel(const __grid_cons
     }
     __syncwarp();
     cluster_sync();
-    if (epi && start && n < p.N) {
-      // CTA r of the cluster adds and stores tokens r, r + split, ... (its two warp groups in turn): parts in the order
-      // of K
-      for (int i = crank + split * ((warp - 2) / 4); i < tokens; i += 2 * split) {
-        float v = 0.0f;
-        for (int q = 0; q < split; ++q) {
-          float part;
-          asm volatile("ld.shared::cluster.f32 %0, [%1];"
-                       : "=f"(part)
-                       : "r"(mapa_shared(smem0 + static_cast<uint32_t>((i * BLK + col) * 4), static_cast<uint32_t>(q)))
-                       : "memory");
-          v += part;
+    // CTA r of the cluster adds and stores tokens r, r + split, ..., a warp each, four weight rows per thread.  All parts'
+    // loads are on their way before the first is added (64 x 5,120 x 5,120: 11.4 us, one load at a time 12.8); added in the
+    // order of K
+    const int64_t n4 = static_cast<int64_t>(nb) * BLK + 4 * lane;
+    if (epi && start && n4 < p.N) {
+      float b4[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) b4[j] = p.bias != nullptr && n4 + j < p.N ? __bfloat162float(p.bias[n4 + j]) : 0.0f;
+      for (int i = crank + split * (warp - 2); i < tokens; i += EPI_WARPS * split) {
+        float part[MAX_SPLIT][4];
+#pragma unroll
+        for (int q = 0; q < MAX_SPLIT; ++q)
+          if (q < split)
+            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                         : "=f"(part[q][0]), "=f"(part[q][1]), "=f"(part[q][2]), "=f"(part[q][3])
+                         : "r"(mapa_shared(smem0 + static_cast<uint32_t>((i * BLK + 4 * lane) * 4), static_cast<uint32_t>(q)))
+                         : "memory");
+        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int q = 0; q < MAX_SPLIT; ++q)
+          if (q < split)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] += part[q][j];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] += b4[j];
+        uint16_t* dst = p.y + (t0 + i) * p.ldy + n4;
+        if (p.vec_out && n4 + 4 <= p.N) {
+          *reinterpret_cast<uint2*>(dst) = make_uint2(to_out2(v[0], v[1], p.out_f16), to_out2(v[2], v[3], p.out_f16));
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (n4 + j < p.N) dst[j] = to_out(v[j], p.out_f16);
         }
-        p.y[(t0 + i) * p.ldy + n] = to_out(v + bias, p.out_f16);
       }
     }
   }
@@ -916,6 +944,7 @@ int launch_narrow(Params& p, const CUtensorMap& tmA, const CUtensorMap& tmW, int
   const int rc = pick_split(fits, kernel, kernel, narrow::THREADS, narrow::smem(NT), 1, narrow::CTAS_PER_SM, dev, token_tiles * p.num_nb, p.num_kb,
                             narrow::ROUND_COST, false, &p.split, &fit, &cost);
   if (rc) return rc;
+  p.vec_out = (reinterpret_cast<uintptr_t>(p.y) & 7u) == 0 && p.ldy % 4 == 0;
   void* args[] = {const_cast<CUtensorMap*>(&tmA), const_cast<CUtensorMap*>(&tmW), &p};
   return launch(kernel, dim3(static_cast<unsigned>(p.num_nb * p.split), static_cast<unsigned>(token_tiles), 1),
                 narrow::THREADS, narrow::smem(NT), p.split, args, st, nullptr);

@@ -176,6 +176,48 @@ def cases(M: int, dev):
         return lambda: ops.fp8_gemm_gate(a, w, sa, sb, x, gate, idx)
     add("fp8_gemm fc2 + indexed gated residual", "tensor", 2.0 * mf * HIDDEN * FFN, s_fc2)
 
+    def s_qb():
+        x = _rand((M, HIDDEN), BF16, g, dev)
+        return lambda: ops.quant_blocks(x)
+    add("quant_blocks (x quant, 128-value blocks)", "hbm", 3 * M * HIDDEN + M * HIDDEN // 32, s_qb)
+
+    def s_sqb():
+        x = _rand((mf, 2 * FFN), BF16, g, dev)
+        return lambda: ops.silu_mul_quant_blocks(x)
+    add("silu_mul_quant_blocks", "hbm", 5 * mf * FFN + mf * FFN // 32, s_sqb)
+
+    def s_qwb():
+        w = _rand((3 * HEADS * D, HIDDEN), BF16, g, dev, 0.02)
+        return lambda: ops.quant_weight_blocks(w)
+    add("quant_weight_blocks (qkv weight, 128 x 128 tiles)", "hbm", 3 * 3 * HEADS * D * HIDDEN, s_qwb)
+
+    def s_gb():
+        a, sa = ops.quant_blocks(_rand((M, HIDDEN), BF16, g, dev))
+        w, sb = ops.quant_weight_blocks(_rand((3 * HEADS * D, HIDDEN), BF16, g, dev, 0.02))
+        return lambda: ops.fp8_gemm_blocks(a, w, sa, sb)
+    add("fp8_gemm_blocks qkv", "tensor", 2.0 * M * 3 * HEADS * D * HIDDEN, s_gb)
+
+    def s_gb1():
+        a, sa = ops.quant_blocks(_rand((1, HIDDEN), BF16, g, dev))
+        ws = [ops.quant_weight_blocks(_rand((3 * HEADS * D, HIDDEN), BF16, g, dev, 0.02)) for _ in range(4)]
+        state = {"i": 0}
+
+        def run():                              # four weights in turn: 315 MB, past the L2
+            state["i"] += 1
+            w, sb = ws[state["i"] % 4]
+            return ops.fp8_gemm_blocks(a, w, sa, sb)
+        return run
+    add("fp8_gemm_blocks qkv, one row", "hbm", 3 * HEADS * D * HIDDEN, s_gb1)
+
+    def s_gg():
+        e, n = 16, 2 * FFN // 16                # the FFN's fc1, cut into 16 experts; rows spread unevenly over them
+        a, sa = ops.quant_blocks(_rand((mf, HIDDEN), BF16, g, dev))
+        w, sb = ops.quant_weight_blocks(_rand((e, n, HIDDEN), BF16, g, dev, 0.02))
+        cuts = torch.randint(0, mf + 1, (e - 1,), device=dev, generator=g).sort().values
+        off = torch.cat([cuts.new_zeros(1), cuts, cuts.new_full((1,), mf)])
+        return lambda: ops.fp8_gemm_grouped(a, w, sa, sb, off)
+    add("fp8_gemm_grouped, 16 experts", "tensor", 2.0 * mf * (2 * FFN // 16) * HIDDEN, s_gg)
+
     def s_sig():
         flags = torch.zeros(8, dtype=torch.int32, device=dev)
         state = {"e": 0}

@@ -360,6 +360,34 @@ def test_grouped_bad_bounds_are_recorded(dev, off, rows):
     check_product(y[:10], a[:10], w[0], sa[:10], sb[0])
 
 
+@pytest.mark.parametrize("rows", [20, 480, 560, 9000])
+def test_grouped_overlapping_bounds_are_recorded(dev, rows):
+    """Every second group claims all rows, the ones between are out of order: more row tiles than correct bounds can make
+    (K is split over clusters in the middle cases), no wait that runs out, and the next call works."""
+    a, w, sa, sb = operands(rows, 136, 2048, experts=8)
+    buf = torch.full((rows + 400, 136), 7.0, dtype=BF16, device=dev)
+    assert ops.device_status() == 0
+    off = torch.tensor([0, rows, 0, rows, 0, rows, 0, rows, rows], device=dev)
+    ops.fp8_gemm_grouped(a, w, sa, sb, off, out=buf[200:200 + rows])
+    assert ops.device_status() == -1
+    assert bool((buf[:200] == 7).all()) and bool((buf[200 + rows:] == 7).all())
+    y = ops.fp8_gemm_grouped(a, w, sa, sb, bounds([rows] + [0] * 7))
+    check_product(y, a, w[0], sa, sb[0])
+
+
+@pytest.mark.parametrize("rows", [1, 128 * 70])
+def test_grouped_bad_bounds_behind_the_last_tile(dev, rows):
+    """Good groups that use up all row tiles of the launch, and a bad bound far behind them."""
+    e = 128
+    a, w, sa, sb = operands(rows, 64, 128, experts=e)
+    off = torch.full((e + 1,), rows, dtype=torch.int32, device=dev)
+    off[0], off[e] = 0, rows + 4
+    assert ops.device_status() == 0
+    y = ops.fp8_gemm_grouped(a, w, sa, sb, off)
+    assert ops.device_status() == -1
+    check_product(y, a, w[0], sa, sb[0])
+
+
 @pytest.mark.parametrize("rows", [48, 700])
 def test_grouped_equals_the_dense_product(dev, rows):
     """One expert with all rows: the same bits as the dense product when both take the same form."""
