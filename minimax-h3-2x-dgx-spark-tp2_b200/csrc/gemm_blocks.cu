@@ -415,7 +415,8 @@ __global__ void __launch_bounds__(THREADS, 1)
                                                           to_out2(v[4], v[5], p.out_f16), to_out2(v[6], v[7], p.out_f16));
           }
           const int64_t nh = n0 + 64 * h;
-          if (whole) {
+          // a TMA store ends at the map's edge rounded up to 16 bytes: slices across an odd edge leave row by row
+          if (whole && (nh + 64 <= p.N || p.N % 8 == 0)) {
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0 && nh < p.N) {
@@ -446,13 +447,14 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       if (p.tma_out && lane == 0) bulk_wait_all0();  // this warp's TMA stores are complete before the CTA leaves
       if constexpr (SPLIT) {
-        // the parts' sums through the idle rings, [256 columns][128 rows] fp32 each; part r adds and stores the groups
+        // the parts' sums through the idle rings, [64][128 rows][4 columns] fp32 each; part r adds and stores the groups
         // r, r + split, ... of 16 columns, the parts in the order of K
         __syncthreads();  // every load has landed and every MMA has read the ring
-        float* sums = reinterpret_cast<float*>(smem);
+        float4* sums = reinterpret_cast<float4*>(smem);
         if (have) {
 #pragma unroll
-          for (int i = 0; i < 128; ++i) sums[(half * 128 + i) * BM + sub * 32 + lane] = acc[i];
+          for (int i = 0; i < 32; ++i)
+            sums[(half * 32 + i) * BM + sub * 32 + lane] = make_float4(acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]);
         }
         __syncwarp();
         cluster_sync();
@@ -464,14 +466,25 @@ __global__ void __launch_bounds__(THREADS, 1)
             float v[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) v[i] = 0.0f;
-            for (int q = 0; q < p.split; ++q) {
-              const uint32_t src = mapa_shared(smem0 + static_cast<uint32_t>((16 * g * BM + sub * 32 + lane) * 4),
-                                               static_cast<uint32_t>(CTAS * q + crank));
+            for (int q0 = 0; q0 < p.split; q0 += 4) {  // four parts' loads on their way at once
+              float x[4][16];
 #pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                float x;
-                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(src + 4u * BM * i) : "memory");
-                v[i] += x;
+              for (int q = 0; q < 4; ++q) {
+                if (q0 + q >= p.split) continue;
+                const uint32_t src = mapa_shared(smem0 + static_cast<uint32_t>((4 * g * BM + sub * 32 + lane) * 16),
+                                                 static_cast<uint32_t>(CTAS * (q0 + q) + crank));
+#pragma unroll
+                for (int i = 0; i < 16; i += 4)
+                  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                               : "=f"(x[q][i]), "=f"(x[q][i + 1]), "=f"(x[q][i + 2]), "=f"(x[q][i + 3])
+                               : "r"(src + 4u * BM * i)
+                               : "memory");
+              }
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                if (q0 + q >= p.split) continue;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) v[i] += x[q][i];
               }
             }
             uint16_t* dst = p.y + m * p.ldy + n;
@@ -894,63 +907,10 @@ int pick_split(Fit<MAX>& fits, const void* whole, const void* parts, int threads
   return H3B_OK;
 }
 
-// a wide launch as planned: which kernels, over how many tiles, in how many parts of K
-template <bool PAIR>
-struct WidePlan {
-  int64_t tiles = 0;  // that there can be
-  int split = 1, fit = 0;
-  double cost = 0;    // in steps
-
-  static const void* whole() { return reinterpret_cast<const void*>(wide::kernel<PAIR, false>); }
-  static const void* parts() { return reinterpret_cast<const void*>(wide::kernel<PAIR, true>); }
-  // T rows in at most `active` groups of `experts`
-  int make(const Params& p, int64_t active, int dev) {
-    static Fit<PAIR ? wide::MAX_SPLIT / 2 : wide::MAX_SPLIT> fits;
-    constexpr int64_t ROWS = PAIR ? 2 * wide::BM : wide::BM;
-    tiles = (p.T + active * (ROWS - 1)) / ROWS * p.num_nb;
-    // to expect: T / ROWS and, where there are several groups, half a row block more for each
-    int64_t expected = p.experts == 1 ? tiles : (p.T + active * ROWS / 2) / ROWS * p.num_nb;
-    if (expected < 1) expected = 1;
-    return pick_split(fits, whole(), parts(), wide::THREADS, wide::SMEM, PAIR ? 2 : 1, 1, dev, expected, p.num_kb,
-                      wide::ROUND_COST, true, &split, &fit, &cost);
-  }
-  int go(Params& p, const CUtensorMap& tmA, const CUtensorMap& tmW, cudaStream_t st) {
-    p.split = split;
-    CUtensorMap tmY = tmA;  // a valid map where no TMA store is made
-    p.vec_out = al16(p.y) && p.ldy % 8 == 0;
-    if (p.vec_out) {
-      const uint64_t dims[2] = {static_cast<uint64_t>(p.N), static_cast<uint64_t>(p.T)};
-      const uint64_t strides[1] = {static_cast<uint64_t>(p.ldy) * 2};
-      const uint32_t box[2] = {64, 32};
-      const int rc = encode_tmap(&tmY, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, p.y, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
-      if (rc) return rc;
-      p.tma_out = 1;
-    }
-    // one part: as many CTAs (pairs) as run at once walk the tiles; more: a cluster for every tile that there can be
-    const int64_t clusters = split == 1 && tiles > fit ? fit : tiles;
-    const int cluster = (PAIR ? 2 : 1) * split;
-    void* args[] = {const_cast<CUtensorMap*>(&tmA), const_cast<CUtensorMap*>(&tmW), &tmY, &p};
-    return launch(split == 1 ? whole() : parts(), dim3(static_cast<unsigned>(cluster * clusters), 1, 1), wide::THREADS,
-                  wide::SMEM, cluster, args, st, nullptr);
-  }
-};
-
-template <int NT>
-int launch_narrow(Params& p, const CUtensorMap& tmA, const CUtensorMap& tmW, int64_t token_tiles, int dev, cudaStream_t st) {
-  static Fit<narrow::MAX_SPLIT> fits;
-  const void* kernel = reinterpret_cast<const void*>(narrow::kernel<NT>);
-  int fit = 0;
-  double cost = 0;
-  const int rc = pick_split(fits, kernel, kernel, narrow::THREADS, narrow::smem(NT), 1, narrow::CTAS_PER_SM, dev, token_tiles * p.num_nb, p.num_kb,
-                            narrow::ROUND_COST, false, &p.split, &fit, &cost);
-  if (rc) return rc;
-  p.vec_out = (reinterpret_cast<uintptr_t>(p.y) & 7u) == 0 && p.ldy % 4 == 0;
-  void* args[] = {const_cast<CUtensorMap*>(&tmA), const_cast<CUtensorMap*>(&tmW), &p};
-  return launch(kernel, dim3(static_cast<unsigned>(p.num_nb * p.split), static_cast<unsigned>(token_tiles), 1),
-                narrow::THREADS, narrow::smem(NT), p.split, args, st, nullptr);
-}
-
 constexpr double SINGLE_STEP = 1.05;  // a step of single CTAs against one of pairs
+// what a call of the wide form takes longer, in steps, than ROUND_COST says of both: it joins four times the sums.  100 x 1,024
+// x 5,120: 8.9 us narrow, 13.6 wide (costs 25 and 19); 65 x 5,120 x 5,120: 14.7 and 14.0 (34 and 20)
+constexpr double NARROW_LEAD = 12;
 
 struct Operands {
   const void* a;
@@ -969,6 +929,89 @@ struct Operands {
   int64_t T, N, K, E;
   int out_dtype;
 };
+
+// a launch as planned: which kernels, over how many tiles, in how many parts of K
+struct Plan {
+  int num_nb = 0;     // column tiles
+  int64_t tiles = 0;  // that there can be
+  int split = 1, fit = 0;
+  double cost = 0;    // in steps
+};
+
+template <bool PAIR>
+struct WidePlan : Plan {
+  static const void* whole() { return reinterpret_cast<const void*>(wide::kernel<PAIR, false>); }
+  static const void* parts() { return reinterpret_cast<const void*>(wide::kernel<PAIR, true>); }
+  // T rows in at most `active` groups
+  int make(const Params& p, int64_t active, int dev) {
+    static Fit<PAIR ? wide::MAX_SPLIT / 2 : wide::MAX_SPLIT> fits;
+    constexpr int64_t ROWS = PAIR ? 2 * wide::BM : wide::BM;
+    num_nb = static_cast<int>((p.N + wide::BN - 1) / wide::BN);
+    tiles = (p.T + active * (ROWS - 1)) / ROWS * num_nb;
+    // to expect: T / ROWS and, where there are several groups, half a row block more for each
+    int64_t expected = p.experts == 1 ? tiles : (p.T + active * ROWS / 2) / ROWS * num_nb;
+    if (expected < 1) expected = 1;
+    return pick_split(fits, whole(), parts(), wide::THREADS, wide::SMEM, PAIR ? 2 : 1, 1, dev, expected, p.num_kb,
+                      wide::ROUND_COST, true, &split, &fit, &cost);
+  }
+  int go(Params& p, const Operands& o, const CUtensorMap& tmW, cudaStream_t st) {
+    p.num_nb = num_nb;
+    p.split = split;
+    CUtensorMap tmA;
+    int rc = load_map(&tmA, o.a, o.K, o.T, o.lda, wide::BM);
+    if (rc) return rc;
+    CUtensorMap tmY = tmA;  // a valid map where no TMA store is made
+    p.vec_out = al16(p.y) && p.ldy % 8 == 0;
+    if (p.vec_out) {
+      const uint64_t dims[2] = {static_cast<uint64_t>(p.N), static_cast<uint64_t>(p.T)};
+      const uint64_t strides[1] = {static_cast<uint64_t>(p.ldy) * 2};
+      const uint32_t box[2] = {64, 32};
+      rc = encode_tmap(&tmY, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, p.y, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+      if (rc) return rc;
+      p.tma_out = 1;
+    }
+    // one part: as many CTAs (pairs) as run at once walk the tiles; more: a cluster for every tile that there can be
+    const int64_t clusters = split == 1 && tiles > fit ? fit : tiles;
+    const int cluster = (PAIR ? 2 : 1) * split;
+    void* args[] = {&tmA, const_cast<CUtensorMap*>(&tmW), &tmY, &p};
+    return launch(split == 1 ? whole() : parts(), dim3(static_cast<unsigned>(cluster * clusters), 1, 1), wide::THREADS,
+                  wide::SMEM, cluster, args, st, nullptr);
+  }
+};
+
+template <int NT>
+struct NarrowPlan : Plan {
+  int64_t token_tiles = 0;
+  int make(const Params& p, int64_t active, int dev) {
+    static Fit<narrow::MAX_SPLIT> fits;
+    num_nb = static_cast<int>((p.N + BLK - 1) / BLK);
+    token_tiles = (p.T + active * (NT - 1)) / NT;
+    tiles = token_tiles * num_nb;
+    if (token_tiles > 65535) return fail(H3B_EUNSUPPORTED, "fp8_gemm_grouped: %lld row tiles of %d", (long long)token_tiles, NT);
+    const void* kernel = reinterpret_cast<const void*>(narrow::kernel<NT>);
+    return pick_split(fits, kernel, kernel, narrow::THREADS, narrow::smem(NT), 1, narrow::CTAS_PER_SM, dev, tiles, p.num_kb,
+                      narrow::ROUND_COST, false, &split, &fit, &cost);
+  }
+  int go(Params& p, const Operands& o, const CUtensorMap& tmW, cudaStream_t st) {
+    p.num_nb = num_nb;
+    p.split = split;
+    p.vec_out = (reinterpret_cast<uintptr_t>(p.y) & 7u) == 0 && p.ldy % 4 == 0;
+    CUtensorMap tmA;
+    const int rc = load_map(&tmA, o.a, o.K, o.T, o.lda, NT);
+    if (rc) return rc;
+    void* args[] = {&tmA, const_cast<CUtensorMap*>(&tmW), &p};
+    return launch(reinterpret_cast<const void*>(narrow::kernel<NT>),
+                  dim3(static_cast<unsigned>(num_nb * split), static_cast<unsigned>(token_tiles), 1), narrow::THREADS,
+                  narrow::smem(NT), split, args, st, nullptr);
+  }
+};
+
+template <int NT>
+int launch_narrow(Params& p, const Operands& o, const CUtensorMap& tmW, int64_t active, int dev, cudaStream_t st) {
+  NarrowPlan<NT> plan;
+  const int rc = plan.make(p, active, dev);
+  return rc ? rc : plan.go(p, o, tmW, st);
+}
 
 int gemm_blocks(const char* what, const Operands& o, cudaStream_t st) {
   const int64_t most = (1ll << 31) - 1;
@@ -1012,37 +1055,40 @@ int gemm_blocks(const char* what, const Operands& o, cudaStream_t st) {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= MAX_DEVICES) return fail(H3B_EUNSUPPORTED, "%s: device ordinal %d", what, dev);
 
-  CUtensorMap tmA, tmW;
+  CUtensorMap tmW;
   int rc = weight_map(&tmW, o.w, o.K, o.N, o.E, o.ldw, o.E > 1 ? o.w_exp : o.ldw * ((o.N + 15) / 16 * 16));
   if (rc) return rc;
-  // groups that can hold a row, and the row tiles that they can need at most
-  const int64_t active = o.T < o.E ? o.T : o.E;
+  const int64_t active = o.T < o.E ? o.T : o.E;  // groups that can hold a row
   const int64_t mean = (o.T + o.E - 1) / o.E;
-  if (mean > 64) {
-    p.num_nb = static_cast<int>((o.N + wide::BN - 1) / wide::BN);
-    if (active > most / p.num_nb || o.T / wide::BM + active > most / (2 * wide::MAX_SPLIT) / p.num_nb)
-      return fail(H3B_EUNSUPPORTED, "%s: 2^31 tiles or more", what);
-    rc = load_map(&tmA, o.a, o.K, o.T, o.lda, wide::BM);
-    if (rc) return rc;
-    // CTA pairs read less (32 KB a step and SM instead of 48) and win by about 8 % where both take as many rounds; single
-    // CTAs, with tiles of half the rows, fit small and ragged work better: 777 x 5,120 x 13,824 in 64 us against 113
+  const int64_t narrow_nb = (o.N + BLK - 1) / BLK, wide_nb = (o.N + wide::BN - 1) / wide::BN;
+  if (o.T / 16 + active > most / narrow_nb || o.T / wide::BM + active > most / (2 * wide::MAX_SPLIT) / wide_nb ||
+      narrow_nb > most / narrow::MAX_SPLIT)
+    return fail(H3B_EUNSUPPORTED, "%s: 2^31 tiles or more", what);
+  // Few rows a group: narrow.  Dense, 64 x 15,360 x 5,120: 20.7 us narrow, 24.4 wide; grouped, uneven groups of 20 rows
+  // in the mean (32 experts of 2,048 x 5,120): 75 and 102; of 38: 88 and 69, of 60: 101 and 69.
+  if (mean > (o.E > 1 ? 32 : 64)) {
     WidePlan<true> pairs;
     WidePlan<false> singles;
     rc = pairs.make(p, active, dev);
     if (!rc) rc = singles.make(p, active, dev);
     if (rc) return rc;
-    return pairs.cost <= SINGLE_STEP * singles.cost ? pairs.go(p, tmA, tmW, st) : singles.go(p, tmA, tmW, st);
+    // CTA pairs read less (32 KB a step and SM instead of 48) and win by a few per cent where both take as many rounds (1,024
+    // x 27,648 x 5,120: 146 us, singles 152); single CTAs, with tiles of half the rows, fit small and ragged work better:
+    // 777 x 5,120 x 13,824 in 65 us against 115
+    const bool paired = pairs.cost <= SINGLE_STEP * singles.cost;
+    if (o.E == 1 && (o.T + 63) / 64 <= 65535) {
+      NarrowPlan<64> few;
+      rc = few.make(p, active, dev);
+      if (rc) return rc;
+      if (few.cost <= (paired ? pairs.cost : singles.cost) + NARROW_LEAD) return few.go(p, o, tmW, st);
+    }
+    return paired ? pairs.go(p, o, tmW, st) : singles.go(p, o, tmW, st);
   }
-  const int nt = mean <= 16 ? 16 : (mean <= 32 ? 32 : 64);
-  p.num_nb = static_cast<int>((o.N + BLK - 1) / BLK);
-  const int64_t token_tiles = (o.T + active * (nt - 1)) / nt;
-  if (token_tiles > 65535) return fail(H3B_EUNSUPPORTED, "%s: %lld row tiles", what, (long long)token_tiles);
-  if (static_cast<int64_t>(p.num_nb) * narrow::MAX_SPLIT > most) return fail(H3B_EUNSUPPORTED, "%s: 2^31 tiles or more", what);
-  rc = load_map(&tmA, o.a, o.K, o.T, o.lda, static_cast<uint32_t>(nt));
-  if (rc) return rc;
-  if (nt == 16) return launch_narrow<16>(p, tmA, tmW, token_tiles, dev, st);
-  if (nt == 32) return launch_narrow<32>(p, tmA, tmW, token_tiles, dev, st);
-  return launch_narrow<64>(p, tmA, tmW, token_tiles, dev, st);
+  // the rows of a tile that is mostly absent cost little but not nothing: 1 x 5,120 x 5,120 takes 8.1 us with tiles of 16
+  // rows, 11.1 with 64; 32 x 5,120 x 13,824 18.5 us with 32 and 19.8 with 64
+  if (mean <= 16) return launch_narrow<16>(p, o, tmW, active, dev, st);
+  if (mean <= 32) return launch_narrow<32>(p, o, tmW, active, dev, st);
+  return launch_narrow<64>(p, o, tmW, active, dev, st);
 }
 
 }  // namespace

@@ -284,6 +284,50 @@ def test_product_nan_stays_in_its_row(dev, m):
     assert torch.equal(y[1:m - 1], want[1:m - 1])
 
 
+# many columns: the wide form with single CTAs (300, 65 rows), with pairs (512, 2,000) and with K in parts (100, 200, 513)
+WIDE = [(300, 20001, 272), (65, 40000, 144), (512, 9400, 512), (2000, 9999, 400), (100, 5120, 5120), (200, 5128, 5120),
+        (513, 2568, 9216)]
+
+
+@pytest.mark.parametrize("out_dtype", [BF16, F16])
+@pytest.mark.parametrize("m,n,k", WIDE)
+def test_wide_product_bias_and_outputs(dev, m, n, k, out_dtype):
+    a, w, sa, sb = operands(m, n, k, seed=3)
+    bias = (torch.randn(n, device=dev, generator=gen(1)) * 3).to(BF16)
+    want = ops.fp8_gemm_blocks(a, w, sa, sb, bias, out_dtype)
+    check_product(want, a, w, sa, sb, bias)
+    for ld, first in ((n + 24 - n % 8, 8), (n + 13, 3)):                             # aligned rows, odd rows
+        buf = torch.full((m + 2, ld), 7.0, dtype=out_dtype, device=dev)
+        out = buf[1:m + 1, first:first + n]
+        ops.fp8_gemm_blocks(a, w, sa, sb, bias, out=out)
+        assert torch.equal(out, want)
+        out.fill_(7.0)
+        assert bool((buf == 7).all())
+
+
+@pytest.mark.parametrize("m,n,k", WIDE)
+def test_wide_product_is_exact_on_integers(dev, m, n, k):
+    g = gen(m)
+    a = torch.randint(-2, 3, (m, k), device=dev, generator=g).float().to(E4M3)
+    w = torch.randint(-2, 3, (n, k), device=dev, generator=g).float().to(E4M3)
+    sa = torch.exp2(torch.randint(-1, 2, (m, nb(k)), device=dev, generator=g).float())
+    sb = torch.exp2(torch.randint(-1, 2, (nb(n), nb(k)), device=dev, generator=g).float())
+    ref = (a.double() * spread(sa.double(), k, 1)) @ (w.double() * spread(spread(sb.double(), n, 0), k, 1)).t()
+    assert torch.equal(ops.fp8_gemm_blocks(a, w, sa, sb), ref.to(BF16))
+
+
+@pytest.mark.parametrize("m,n,k", WIDE)
+def test_wide_product_nan_stays_in_its_row(dev, m, n, k):
+    a, w, sa, sb = operands(m, n, k, seed=2)
+    want = ops.fp8_gemm_blocks(a, w, sa, sb)
+    a2, sa2 = a.clone(), sa.clone()
+    a2.view(torch.uint8)[0, 5] = 0x7F
+    sa2[m - 1, 1] = float("nan")
+    y = ops.fp8_gemm_blocks(a2, w, sa2, sb)
+    assert bool(torch.isnan(y[0]).all()) and bool(torch.isnan(y[m - 1]).all())
+    assert torch.equal(y[1:m - 1], want[1:m - 1])
+
+
 def test_product_repeats_bit_for_bit(dev):
     for m, n, k in ((1, 512, 5120), (40, 1024, 4096), (600, 1024, 2048)):
         a, w, sa, sb = operands(m, n, k, seed=m)
