@@ -5,14 +5,25 @@
 //
 // The scales change every 128 values of K, so the tensor core's accumulator holds one block's product only: each
 // K step of 128 is its own accumulator in TMEM, and the epilogue warps add it, scaled, to fp32 running sums in
-// registers while the next step's MMAs fill the other TMEM buffer.  Both forms below are that loop:
+// registers while the next step's MMAs fill another TMEM buffer.  Both forms below are that loop:
 //
-//   wide    (over 64 rows a group): CTA pairs with 2-SM MMAs over 256 rows x 256 columns.  Thread = output row, so sa * sb is one
-//           scalar per thread and step and the promotion costs one FMA per element: 8 warps x 128 FMAs per 512 tensor
-//           cycles.  128 running sums per thread, two 256-column TMEM buffers.
+//   wide    (many rows): CTA pairs with 2-SM MMAs over 256 rows x 256 columns, or single CTAs over 128 x 256.  Thread = output
+//           row, so sa * sb is one scalar per thread and step and the promotion costs one FMA per element: 8 warps x 128 FMAs
+//           per 512 tensor cycles.  128 running sums per thread, two 256-column TMEM buffers.
 //   narrow  (few rows): the operands swapped, D^T = w a^T: 128 weight rows x NT tokens (NT = 16, 32 or 64) per CTA, so that
-//           a tile streams the weight once with no tensor work on absent rows.  K is split over a cluster of CTAs that
-//           add their sums through distributed shared memory in a fixed order (the result does not depend on timing).
+//           a tile streams the weight once with no tensor work on absent rows.
+//
+// Where the tiles are few, K is split over a cluster of CTAs that add their sums through distributed shared memory in the
+// order of K (the result does not depend on timing).
+//
+// What bounds them.  Wide, 62,496 x 15,360 x 5,120: 5.0 to 5.4 ms, 1.9 PFLOP/s, at the power cap (about 1.5 GHz); the tensor
+// pipe alone would take 512 cycles a step, a step takes about 1,000.  A TMEM buffer goes round between the MMAs, the eight
+// epilogue warps (of both SMs) and back: 512 cycles of MMAs, then commit, TMEM reads under the additions and the arrival,
+// 1,200 more where the other SM is part of it, and 512 columns hold only two buffers.  Half as wide buffers, four of them:
+// 6.1 ms (twice the handshakes).  Sixteen epilogue warps of 64 columns: 7.7 ms.  Two additions per instruction (fma.rn.f32x2):
+// fewer cycles alone, more here.  Single CTAs have no cross-SM handshake, but read 48 KB a step and SM and meet the L2's limit
+// (about 12 TB/s) at the same speed.  Narrow: the weight's bytes, and at one row the start and end of a call: 1 x 15,360 x
+// 5,120 16.7 us (12.2 at copy speed), 1 x 5,120 x 5,120 8.1 (4.1).
 //
 // Every wait is bounded (common.cuh); no TMA multicast.
 #include <atomic>
@@ -120,7 +131,7 @@ __device__ __forceinline__ bool cluster_flag(uint32_t flag_smem) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// wide: CTA pairs, 256 x 256 tiles, running sums in registers
+// wide: 256 x 256 tiles by CTA pairs or 128 x 256 by single CTAs, running sums in registers
 // ---------------------------------------------------------------------------------------------------------------
 namespace wide {
 
@@ -131,11 +142,15 @@ __host__ __device__ constexpr int stage_bytes(bool pair) { return (BM + (pair ? 
 constexpr int RING_BYTES = stages(true) * stage_bytes(true);
 static_assert(RING_BYTES == stages(false) * stage_bytes(false), "the rings take the same room");
 constexpr int EPI_WARPS = 8, FIRST_EPI = 4, THREADS = 32 * (FIRST_EPI + EPI_WARPS);
-constexpr int MAX_SPLIT = 8, ROUND_COST = 14;        // clusters of 8 CTAs at most: 4 parts for pairs
+// Clusters of 8 CTAs at most: 4 parts for pairs.  What a round of tiles takes besides its steps, in steps: with 7 or less, 512
+// x 5,120 x 5,120 goes to 2 rounds in parts, 37 us for 26; at 28 nothing measured changed.  Without parts 256 x 1,024 x 13,824
+// takes 53 us for 21, 256 x 5,120 x 13,824 57 for 33
+constexpr int MAX_SPLIT = 8, ROUND_COST = 14;
 constexpr int WARP_STAGING = 32 * 128;              // 32 rows x 64 columns of 16-bit output
 constexpr int SMEM = RING_BYTES + 1024 + 1024 + EPI_WARPS * WARP_STAGING;
 static_assert(SMEM <= 232448, "shared memory");
-// row blocks (256 rows) that share a column block's w tile in L2, as in the per-token product
+// row blocks that share a column block's w tile in L2, as in the per-token product (4 and 8 measure the same, 32 takes 3 %
+// longer at 8,192 x 15,360 x 5,120)
 constexpr int GROUP_M = 16;
 
 // tile r of a group of `blocks` row blocks -> (row block, column block)
@@ -202,7 +217,8 @@ __global__ void __launch_bounds__(THREADS, 1)
   if (threadIdx.x == 0) *start_flag = status_bad(p.wc) ? 0u : 1u;
   tc_fence_before();
   cluster_sync();
-  tc_fence_after();  // no pdl_launch in this form: the next kernel starting as CTAs leave cost an FFN chain of 256 rows 3 of 89 us
+  tc_fence_after();
+  // no pdl_launch in this form: with the next kernel starting as CTAs leave, an FFN chain of 256 rows takes 92 us for 89
   const uint32_t tmem_base = *tmem_slot;
   const bool start = cluster_flag(smem_u32(start_flag));  // of the cluster's first CTA
   const int first_tile = static_cast<int>(cluster_id_x()), tile_step = static_cast<int>(cluster_count_x());
@@ -454,7 +470,8 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (have) {
 #pragma unroll
           for (int i = 0; i < 32; ++i)
-            sums[(half * 32 + i) * BM + sub * 32 + lane] = make_float4(acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]);
+            sums[(half * 32 + i) * BM + sub * 32 + lane] =
+                make_float4(acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]);
         }
         __syncwarp();
         cluster_sync();
@@ -536,6 +553,8 @@ namespace narrow {
 constexpr int EPI_WARPS = 8, EPI_THREADS = 32 * EPI_WARPS;
 constexpr int THREADS = 64 + EPI_THREADS;  // producer, MMA issuer, epilogue (4 row quarters x 2 token halves)
 constexpr int CHUNK = 16;                  // K steps whose scales are staged together
+// as in the wide form: with 0, 48 rows over 64 experts of 4,096 x 5,120 take 118 us for 105 (10 and 40: 105).  Without parts
+// 1 x 5,120 x 5,120 takes 16.6 us for 8.2, 16 x 5,120 x 13,824 40 for 17
 constexpr int MAX_SPLIT = 8, ROUND_COST = 20;
 constexpr int NBUF = 4;                    // TMEM buffers of NT columns: steps between the MMAs and the epilogue
 
@@ -659,7 +678,9 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) kernel(const __grid_cons
         uint32_t phase = 0, it = 0;
         for (int kb = kb0; kb < kb1; ++kb, ++it) {
           const int b = it % NBUF;
-          if (!mbar_wait_inline(full_bar(stage), phase, p.wc) || !mbar_wait_inline(tempty_bar(b), ((it / NBUF) & 1u) ^ 1u, p.wc)) break;
+          if (!mbar_wait_inline(full_bar(stage), phase, p.wc) ||
+              !mbar_wait_inline(tempty_bar(b), ((it / NBUF) & 1u) ^ 1u, p.wc))
+            break;
           tc_fence_after();
           const uint32_t sW = smem0 + stage * STAGE_BYTES;
           const uint64_t wdesc = sdesc_sw128(sW, 16, 1024), adesc = sdesc_sw128(sW + BLK * BLK, 16, 1024);
@@ -851,7 +872,8 @@ int launch(const void* kernel, dim3 grid, int threads, int smem, int cluster, vo
   cfg.attrs = attr;
   cfg.numAttrs = fit != nullptr ? 1 : 2;
   // with `fit`: no launch, but how many such clusters run at once
-  const cudaError_t e = fit != nullptr ? cudaOccupancyMaxActiveClusters(fit, kernel, &cfg) : cudaLaunchKernelExC(&cfg, kernel, args);
+  const cudaError_t e =
+      fit != nullptr ? cudaOccupancyMaxActiveClusters(fit, kernel, &cfg) : cudaLaunchKernelExC(&cfg, kernel, args);
   if (e != cudaSuccess) return cuda_fail(e, fit != nullptr ? "fp8_gemm_blocks: cluster occupancy" : "fp8_gemm_blocks launch");
   return H3B_OK;
 }
@@ -870,7 +892,8 @@ struct Fit {
       e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
     if (e != cudaSuccess) return cuda_fail(e, "fp8_gemm_blocks: shared memory");
     const int cluster = unit * parts;
-    const int rc = launch(kernel, dim3(static_cast<unsigned>(cluster * num_sms()), 1, 1), threads, smem, cluster, nullptr, nullptr, fit);
+    const int rc = launch(kernel, dim3(static_cast<unsigned>(cluster * num_sms()), 1, 1), threads, smem, cluster, nullptr,
+                          nullptr, fit);
     if (rc) return rc;
     *fit *= per_sm;
     if (*fit < 1) *fit = -1;
@@ -883,8 +906,8 @@ struct Fit {
 // a part and `round_cost`, what a round takes besides, in steps.  A persistent grid of single parts pays that once.
 // `whole` / `parts`: the kernels for one part and for more.
 template <int MAX>
-int pick_split(Fit<MAX>& fits, const void* whole, const void* parts, int threads, int smem, int unit, int per_sm, int dev, int64_t tiles, int num_kb,
-               int round_cost, bool persistent, int* split, int* fit1, double* best_cost) {
+int pick_split(Fit<MAX>& fits, const void* whole, const void* parts, int threads, int smem, int unit, int per_sm, int dev,
+               int64_t tiles, int num_kb, int round_cost, bool persistent, int* split, int* fit1, double* best_cost) {
   double& best = *best_cost;
   for (int s = 1; s <= MAX; ++s) {
     if (s > 1 && num_kb < 4 * s) break;  // four steps each at least
@@ -907,7 +930,8 @@ int pick_split(Fit<MAX>& fits, const void* whole, const void* parts, int threads
   return H3B_OK;
 }
 
-constexpr double SINGLE_STEP = 1.05;  // a step of single CTAs against one of pairs
+// a step of single CTAs against one of pairs, whose tiles they choose between: both sides measured at the choice below
+constexpr double SINGLE_STEP = 1.05;
 // what a call of the wide form takes longer, in steps, than ROUND_COST says of both: it joins four times the sums.  100 x 1,024
 // x 5,120: 8.9 us narrow, 13.6 wide (costs 25 and 19); 65 x 5,120 x 5,120: 14.7 and 14.0 (34 and 20)
 constexpr double NARROW_LEAD = 12;
@@ -987,10 +1011,11 @@ struct NarrowPlan : Plan {
     num_nb = static_cast<int>((p.N + BLK - 1) / BLK);
     token_tiles = (p.T + active * (NT - 1)) / NT;
     tiles = token_tiles * num_nb;
-    if (token_tiles > 65535) return fail(H3B_EUNSUPPORTED, "fp8_gemm_grouped: %lld row tiles of %d", (long long)token_tiles, NT);
+    if (token_tiles > 65535)
+      return fail(H3B_EUNSUPPORTED, "fp8_gemm_grouped: %lld row tiles of %d", (long long)token_tiles, NT);
     const void* kernel = reinterpret_cast<const void*>(narrow::kernel<NT>);
-    return pick_split(fits, kernel, kernel, narrow::THREADS, narrow::smem(NT), 1, narrow::CTAS_PER_SM, dev, tiles, p.num_kb,
-                      narrow::ROUND_COST, false, &split, &fit, &cost);
+    return pick_split(fits, kernel, kernel, narrow::THREADS, narrow::smem(NT), 1, narrow::CTAS_PER_SM, dev, tiles,
+                      p.num_kb, narrow::ROUND_COST, false, &split, &fit, &cost);
   }
   int go(Params& p, const Operands& o, const CUtensorMap& tmW, cudaStream_t st) {
     p.num_nb = num_nb;
@@ -1053,7 +1078,8 @@ int gemm_blocks(const char* what, const Operands& o, cudaStream_t st) {
   p.wc.timeout = wait_timeout_ns();
   if (p.wc.status == nullptr) return fail(H3B_ECUDA, "%s: device status word", what);
   int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= MAX_DEVICES) return fail(H3B_EUNSUPPORTED, "%s: device ordinal %d", what, dev);
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= MAX_DEVICES)
+    return fail(H3B_EUNSUPPORTED, "%s: device ordinal %d", what, dev);
 
   CUtensorMap tmW;
   int rc = weight_map(&tmW, o.w, o.K, o.N, o.E, o.ldw, o.E > 1 ? o.w_exp : o.ldw * ((o.N + 15) / 16 * 16));
