@@ -4,12 +4,15 @@
 //   scale = max(amax / 448, 1/(448*512)),  q = e4m3_rn(clamp(h * (1 / scale), -448, 448))     (NaN propagates)
 //
 // Activations: 16 lanes hold a block as one 16-byte load each (8 bf16 values), reduce its abs-max inside the half-warp and
-// write 128 bytes of e4m3; no shared memory, no barrier.  A warp takes the same block of eight consecutive rows: blocks
-// taken along a row instead, each with divisions and a 4-byte scale store of its own, ran at 4.9 TB/s (62,496 x 5,120:
-// 199 us), this at 6.4 (151 us; the copy rate is 6.46).  silu-mul, 31,248 x
-// 13,824: 361 us, 6.0 TB/s (blocks along a row 466; two rows 429; CTAs of 256 threads 385).  Weights: a CTA of 256 threads
-// holds a 128 x 128 tile in registers (8 vectors per thread) and reduces it once: 15,360 x 5,120 in 36 us, 6.5 TB/s (512
-// threads: 50 us).  Every value is read once and written once.
+// write 128 bytes of e4m3; no shared memory, no barrier.  A warp takes the same block of eight consecutive rows (blocks taken
+// along a row instead, each with divisions and a 4-byte scale store of its own, ran at 4.9 TB/s).  Weights: a CTA of 256
+// threads holds a 128 x 128 tile in registers (8 vectors per thread) and reduces it once (512 threads: 50 us for 36).  Every
+// value is read once and written once.
+//
+// Measured in long runs, which sit at the power cap (1.6 GHz): 62,496 x 5,120 in 153 us, 6.3 TB/s (139 us before the cap
+// sets in; a plain copy of as many bytes 148, under the cap); silu-mul, 31,248 x 13,824, 362 us, 6.0 TB/s (312 before); weight
+// 15,360 x 5,120 in 36 us.  Instructions are what the power goes into: with about twice as many the same calls took 168, 401
+// and 39 us.  Load and store hints (evict first, no allocation in L1) measure the same or slower.
 #include "common.cuh"
 #include "quant.cuh"
 
@@ -18,52 +21,99 @@ namespace {
 
 constexpr int BLK = 128;
 
-// 8 values of a row starting at column c, as bf16 bit patterns; VEC: one 16-byte load (K % 8 == 0, so they are all in
-// the row or all past it); otherwise value by value with columns at or past K as zero
-template <bool VEC>
-__device__ __forceinline__ uint4 load8(const uint16_t* row, int64_t c, int64_t K) {
+// 8 bf16 values at x, `left` columns before the row's end, as bit patterns.  ALL: every one is in the row.  VEC: one 16-byte
+// load (K % 8 == 0, so they are all in the row or all past it); otherwise value by value, those past the end as zero
+template <bool VEC, bool ALL>
+__device__ __forceinline__ uint4 load8(const uint16_t* x, int64_t left) {
   if constexpr (VEC) {
-    return c < K ? __ldg(reinterpret_cast<const uint4*>(row + c)) : make_uint4(0, 0, 0, 0);
+    return ALL || left > 0 ? __ldg(reinterpret_cast<const uint4*>(x)) : make_uint4(0, 0, 0, 0);
   } else {
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t lo = c + 2 * i < K ? row[c + 2 * i] : 0u;
-      const uint32_t hi = c + 2 * i + 1 < K ? row[c + 2 * i + 1] : 0u;
+      const uint32_t lo = 2 * i < left ? x[2 * i] : 0u;
+      const uint32_t hi = 2 * i + 1 < left ? x[2 * i + 1] : 0u;
       w[i] = lo | (hi << 16);
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
 
-template <bool VEC>
-__device__ __forceinline__ void store8(uint8_t* row, int64_t c, int64_t K, uint2 v) {
+template <bool VEC, bool ALL>
+__device__ __forceinline__ void store8(uint8_t* q, int64_t left, uint2 v) {
   if constexpr (VEC) {
-    if (c < K) *reinterpret_cast<uint2*>(row + c) = v;
+    if (ALL || left > 0) *reinterpret_cast<uint2*>(q) = v;
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (c + i < K) row[c + i] = static_cast<uint8_t>((i < 4 ? v.x : v.y) >> (8 * (i & 3)));
+      if (i < left) q[i] = static_cast<uint8_t>((i < 4 ? v.x : v.y) >> (8 * (i & 3)));
   }
+}
+
+// Two fp32 operations per instruction.  The large calls run at the power cap, where instructions cost clock: with these, the
+// pointers stepped from row to row and the checks of whole blocks made once, the quantisers issue half as many.
+struct F2 {
+  float lo, hi;
+};
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("{\n\t.reg .b64 ra, rb, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\tmul.rn.f32x2 rd, ra, rb;\n\t"
+      "mov.b64 {%0, %1}, rd;\n\t}"
+      : "=f"(r.lo), "=f"(r.hi)
+      : "f"(a.lo), "f"(a.hi), "f"(b.lo), "f"(b.hi));
+  return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("{\n\t.reg .b64 ra, rb, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\tadd.rn.f32x2 rd, ra, rb;\n\t"
+      "mov.b64 {%0, %1}, rd;\n\t}"
+      : "=f"(r.lo), "=f"(r.hi)
+      : "f"(a.lo), "f"(a.hi), "f"(b.lo), "f"(b.hi));
+  return r;
+}
+__device__ __forceinline__ F2 unpack2(uint32_t w) { return F2{lo_bf16(w), hi_bf16(w)}; }
+
+// larger magnitudes of two bf16 pairs (signs: anything; NaN if either is)
+__device__ __forceinline__ uint32_t absmax2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t absmax_of(const uint4& v) { return absmax2(absmax2(v.x, v.y), absmax2(v.z, v.w)); }
+// the largest magnitude of a pair, as the bits of an fp32 (they order like the magnitudes, NaN above all)
+__device__ __forceinline__ uint32_t absmax_bits(uint32_t m2) { return fold16(m2 & 0x7FFF7FFFu) << 16; }
+
+// x * inv to e4m3, to nearest even; satfinite clamps to +-448 and keeps NaN
+__device__ __forceinline__ uint2 quant8(const F2 (&x)[4], float inv) {
+  uint32_t o[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const F2 a = mul2(x[2 * i], F2{inv, inv}), b = mul2(x[2 * i + 1], F2{inv, inv});
+    o[i] = static_cast<uint32_t>(f32x2_to_e4m3x2(a.lo, a.hi)) | (static_cast<uint32_t>(f32x2_to_e4m3x2(b.lo, b.hi)) << 16);
+  }
+  return make_uint2(o[0], o[1]);
+}
+__device__ __forceinline__ uint2 quant8_bf16(const uint4& v, float inv) {
+  const F2 x[4] = {unpack2(v.x), unpack2(v.y), unpack2(v.z), unpack2(v.w)};
+  return quant8(x, inv);
 }
 
 __device__ __forceinline__ float block_scale(uint32_t amax_bits, int div_mode) {
   return nan_max(qdiv(__uint_as_float(amax_bits), kFp8Max, div_mode), kMinScale);
 }
 
-// silu(g) * u in fp32, not rounded before the quant: one rounding, to e4m3.  The fast exponential and division are within
-// (2 + 1.173 |g|) and 2 units in the last place, i.e. (6 + 1.2 |g|) * 2^-23 in all, against the 2^-4 of the rounding.
-__device__ __forceinline__ float silu_mul_f32(float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; }
-
-__device__ __forceinline__ uint2 quant8f(const float (&y)[8], float inv) {
-  uint32_t o[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint16_t a = f32x2_to_e4m3x2(y[4 * i] * inv, y[4 * i + 1] * inv);
-    const uint16_t b = f32x2_to_e4m3x2(y[4 * i + 2] * inv, y[4 * i + 3] * inv);
-    o[i] = static_cast<uint32_t>(a) | (static_cast<uint32_t>(b) << 16);
-  }
-  return make_uint2(o[0], o[1]);
+// silu(g) * u = g / (1 + 2^(-g log2 e)) * u in fp32, not rounded before the quant: one rounding, to e4m3.  The argument's
+// rounding counts |g| * 0.75, ex2.approx 2, rcp.approx 1 and the other four steps half a unit each: within (5 + 0.75 |g|) *
+// 2^-23 in all, against the 2^-4 of e4m3.  Below g = -87 the reciprocal, under 2^-126, is flushed and silu is 0.
+__device__ __forceinline__ F2 silu_mul2(F2 g, F2 u) {
+  constexpr float NEG_LOG2E = -1.4426950408889634f;
+  F2 e = mul2(g, F2{NEG_LOG2E, NEG_LOG2E});
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e.lo));
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e.hi));
+  F2 r = add2(e, F2{1.0f, 1.0f});
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(r.lo));
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(r.hi));
+  return mul2(mul2(g, r), u);
 }
 
 constexpr int U = 4;  // rows of a half-warp (two: 5.5 TB/s where four make 6.4)
@@ -82,6 +132,57 @@ __device__ __forceinline__ uint32_t half_warp_max(const uint32_t (&v)[U], int hl
   return max(m, __shfl_xor_sync(ALL, m, 1));
 }
 
+// A warp's unit: blocks of 2U consecutive rows at x (the lane's first row and column; SILU: up columns `K` further on), of
+// which this lane's half-warp has U.  `rows`, `left`: rows from the lane's first and columns from the lane's first to the end.
+template <bool VEC, bool SILU, bool ALL>
+__device__ __forceinline__ void quant_unit(const uint16_t* __restrict__ x, int64_t stride_x, int64_t K, int rows,
+                                           int64_t left, uint8_t* __restrict__ q, float* __restrict__ s, int64_t s_row,
+                                           int div_mode) {
+  const int hl = threadIdx.x & 15;
+  uint4 v[U], w[SILU ? U : 1];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    v[u] = make_uint4(0, 0, 0, 0);
+    if (SILU) w[u] = make_uint4(0, 0, 0, 0);
+    if (ALL || u < rows) {
+      v[u] = load8<VEC, ALL>(x, left);
+      if (SILU) w[u] = load8<VEC, ALL>(x + K, left);
+    }
+    x += stride_x;
+  }
+  F2 y[SILU ? U : 1][4];
+  uint32_t amax[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if constexpr (SILU) {
+      const uint32_t g[4] = {v[u].x, v[u].y, v[u].z, v[u].w}, up[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
+      float m = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        y[u][e] = silu_mul2(unpack2(g[e]), unpack2(up[e]));
+        asm("max.NaN.abs.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(y[u][e].lo), "f"(y[u][e].hi));
+      }
+      amax[u] = __float_as_uint(m);
+    } else {
+      amax[u] = absmax_bits(absmax_of(v[u]));
+    }
+  }
+  const float scale = block_scale(half_warp_max(amax, hl), div_mode);
+  const float inv = qdiv(1.0f, scale, div_mode);
+  if (hl % 4 == 0 && (ALL || hl / 4 < rows)) s[hl / 4 * s_row] = scale;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const float inv_u = __shfl_sync(0xffffffffu, inv, (threadIdx.x & 16) + u * 4);
+    if (ALL || u < rows) {
+      if constexpr (SILU)
+        store8<VEC, ALL>(q, left, quant8(y[u], inv_u));
+      else
+        store8<VEC, ALL>(q, left, quant8_bf16(v[u], inv_u));
+    }
+    q += K;
+  }
+}
+
 // rows x [rows, K] (SILU: [rows, 2K], gate | up) -> q [rows, K], s[row * s_row + j * s_blk].  A warp takes block j of 2U
 // consecutive rows, U per half-warp: their scales are then neighbours in the block-major scale tensor and leave in one
 // store, each division is made once per warp for 2U blocks, and the loads of a CTA's 4 warps run along the rows.
@@ -92,55 +193,54 @@ __global__ void __launch_bounds__(128) quant_blocks_kernel(const uint16_t* __res
                                                            int64_t s_blk, int div_mode) {
   pdl_wait();
   pdl_launch();
-  const int hl = threadIdx.x & 15;
   const uint32_t unit = blockIdx.x * 4u + (threadIdx.x >> 5);
   if (unit >= units) return;  // the whole warp
   const uint32_t group = unit / KB, j = unit - group * KB;
-  const uint32_t row0 = group * (2u * U) + (threadIdx.x & 16 ? U : 0u);
-  const int64_t c = static_cast<int64_t>(j) * BLK + hl * 8;
-  uint4 v[U], w[U];
+  const int64_t row0 = static_cast<int64_t>(group) * (2 * U) + (threadIdx.x & 16 ? U : 0);
+  const int64_t c = static_cast<int64_t>(j) * BLK + (threadIdx.x & 15) * 8;
+  x += row0 * stride_x + c;
+  q += row0 * K + c;
+  s += row0 * s_row + j * s_blk;
+  const bool all = (group + 1) * (2 * U) <= rows && (j + 1) * static_cast<int64_t>(BLK) <= K;
+  if (VEC && all)
+    quant_unit<VEC, SILU, VEC>(x, stride_x, K, U, 8, q, s, s_row, div_mode);
+  else
+    quant_unit<VEC, SILU, false>(x, stride_x, K, static_cast<int>(rows) - static_cast<int>(row0), K - c, q, s, s_row,
+                                 div_mode);
+}
+
+// A CTA's tile: rows tile row r0 + 16 u of the lane at w (step_w elements apart), 8 columns each.  `rows`, `left` as above.
+template <bool VEC, bool ALL>
+__device__ __forceinline__ void quant_tile(const uint16_t* __restrict__ w, int64_t step_w, int64_t rows, int64_t left,
+                                           uint8_t* __restrict__ q, int64_t step_q, float* __restrict__ s, int div_mode) {
+  __shared__ uint32_t red[8];
+  __shared__ float tile_scale[2];  // and its inverse
+  uint4 v[8];
+  uint32_t m2 = 0;
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    v[u] = w[u] = make_uint4(0, 0, 0, 0);
-    if (row0 + u < rows) {
-      const uint16_t* xr = x + (row0 + u) * stride_x;
-      v[u] = load8<VEC>(xr, c, K);
-      if (SILU) w[u] = load8<VEC>(xr + K, c, K);
-    }
+  for (int u = 0; u < 8; ++u) {
+    v[u] = ALL || 16 * u < rows ? load8<VEC, ALL>(w, left) : make_uint4(0, 0, 0, 0);
+    m2 = absmax2(m2, absmax_of(v[u]));
+    w += step_w;
   }
-  float y[SILU ? U : 1][8];
-  uint32_t amax[U];
+  const uint32_t wmax = __reduce_max_sync(0xffffffffu, absmax_bits(m2));
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = wmax;
+  __syncthreads();
+  uint32_t amax = red[0];
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    if constexpr (SILU) {
-      float f[8];
-      unpack8(v[u], y[u]);
-      unpack8(w[u], f);
-      amax[u] = 0;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        y[u][e] = silu_mul_f32(y[u][e], f[e]);
-        amax[u] = max(amax[u], __float_as_uint(y[u][e]) & 0x7FFFFFFFu);  // NaN bits sort above every number
-      }
-    } else {
-      amax[u] = fold16(absmax8(v[u], 0)) << 16;
-    }
+  for (int k = 1; k < 8; ++k) amax = max(amax, red[k]);
+  if (threadIdx.x < 32) {  // the divisions in one warp: in all eight they took a tenth of the kernel
+    const float scale = block_scale(amax, div_mode);
+    tile_scale[0] = scale;
+    tile_scale[1] = qdiv(1.0f, scale, div_mode);
   }
-  const float scale = block_scale(half_warp_max(amax, hl), div_mode);
-  const float inv = qdiv(1.0f, scale, div_mode);
-  const uint32_t mine = row0 + hl / 4;
-  if (hl % 4 == 0 && mine < rows) s[mine * s_row + j * s_blk] = scale;
+  __syncthreads();
+  const float inv = tile_scale[1];
+  if (threadIdx.x == 0) *s = tile_scale[0];  // behind the barrier: ahead of it the others waited for it, 39.4 us for 36
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const float inv_u = __shfl_sync(0xffffffffu, inv, (threadIdx.x & 16) + u * 4);
-    if (row0 + u < rows) {
-      uint2 out;
-      if constexpr (SILU)
-        out = quant8f(y[u], inv_u);
-      else
-        out = quant8(v[u], inv_u);
-      store8<VEC>(q + (row0 + u) * K, c, K, out);
-    }
+  for (int u = 0; u < 8; ++u) {
+    if (ALL || 16 * u < rows) store8<VEC, ALL>(q, left, quant8_bf16(v[u], inv));
+    q += step_q;
   }
 }
 
@@ -150,42 +250,19 @@ __global__ void __launch_bounds__(256) quant_weight_blocks_kernel(const uint16_t
                                                                   int64_t stride_e, int64_t stride_n, uint32_t NB,
                                                                   uint32_t KB, uint8_t* __restrict__ q,
                                                                   float* __restrict__ s, int div_mode) {
-  __shared__ uint32_t red[8];
-  __shared__ float tile_scale[2];  // and its inverse
   pdl_wait();
   pdl_launch();
   const uint32_t tile = blockIdx.x;
   const uint32_t j = tile % KB, en = tile / KB, i = en % NB, e = en / NB;
   const int64_t c = static_cast<int64_t>(j) * BLK + (threadIdx.x & 15) * 8;
   const int64_t r0 = static_cast<int64_t>(i) * BLK + (threadIdx.x >> 4);
-  const uint16_t* we = w + e * stride_e;
-  uint4 v[8];
-  uint32_t m2 = 0;
-#pragma unroll
-  for (int u = 0; u < 8; ++u) {
-    const int64_t r = r0 + 16 * u;
-    v[u] = r < N ? load8<VEC>(we + r * stride_n, c, K) : make_uint4(0, 0, 0, 0);
-    m2 = absmax8(v[u], m2);
-  }
-  const uint32_t wmax = __reduce_max_sync(0xffffffffu, fold16(m2));
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = wmax;
-  __syncthreads();
-  uint32_t amax = red[0];
-#pragma unroll
-  for (int k = 1; k < 8; ++k) amax = max(amax, red[k]);
-  if (threadIdx.x < 32) {  // the divisions in one warp: in all eight they took a tenth of the kernel
-    const float scale = block_scale(amax << 16, div_mode);
-    tile_scale[0] = scale;
-    tile_scale[1] = qdiv(1.0f, scale, div_mode);
-  }
-  __syncthreads();
-  const float inv = tile_scale[1];
-  if (threadIdx.x == 0) s[tile] = tile_scale[0];  // behind the barrier: ahead of it the others waited for it, 39.4 us for 36
-#pragma unroll
-  for (int u = 0; u < 8; ++u) {
-    const int64_t r = r0 + 16 * u;
-    if (r < N) store8<VEC>(q + (e * N + r) * K, c, K, quant8(v[u], inv));
-  }
+  w += e * stride_e + r0 * stride_n + c;
+  q += (e * N + r0) * K + c;
+  s += tile;
+  if (VEC && (i + 1) * static_cast<int64_t>(BLK) <= N && (j + 1) * static_cast<int64_t>(BLK) <= K)
+    quant_tile<VEC, VEC>(w, 16 * stride_n, BLK, 8, q, 16 * K, s, div_mode);
+  else
+    quant_tile<VEC, false>(w, 16 * stride_n, N - r0, K - c, q, 16 * K, s, div_mode);
 }
 
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
