@@ -3,16 +3,17 @@
 // those of the per-token quant, taken over a block:
 //   scale = max(amax / 448, 1/(448*512)),  q = e4m3_rn(clamp(h * (1 / scale), -448, 448))     (NaN propagates)
 //
-// Activations: 16 lanes hold a block as one 16-byte load each (8 bf16 values), reduce its abs-max inside the half-warp and
-// write 128 bytes of e4m3; no shared memory, no barrier.  A warp takes the same block of eight consecutive rows (blocks taken
-// along a row instead, each with divisions and a 4-byte scale store of its own, ran at 4.9 TB/s).  Weights: a CTA of 256
-// threads holds a 128 x 128 tile in registers (8 vectors per thread) and reduces it once (512 threads: 50 us for 36).  Every
-// value is read once and written once.
+// Activations: eight lanes hold a block, 16 values each in one 32-byte load, reduce its abs-max by shuffles and write 16 bytes
+// of e4m3 a lane; no shared memory, no barrier.  A warp takes the same block of eight consecutive rows (blocks taken along a
+// row instead, each with divisions and a 4-byte scale store of its own, ran at 4.9 TB/s).  Weights: a CTA of 256 threads
+// holds a 128 x 128 tile in registers and reduces it once (512 threads: 50 us for 36).  Every value is read once and
+// written once.
 //
-// Measured in long runs, which sit at the power cap (1.6 GHz): 62,496 x 5,120 in 153 us, 6.3 TB/s (139 us before the cap
-// sets in; a plain copy of as many bytes 148, under the cap); silu-mul, 31,248 x 13,824, 362 us, 6.0 TB/s (312 before); weight
-// 15,360 x 5,120 in 36 us.  Instructions are what the power goes into: with about twice as many the same calls took 168, 401
-// and 39 us.  Load and store hints (evict first, no allocation in L1) measure the same or slower.
+// Long runs sit at the power cap, where each instruction costs clock, so their number counts although memory bounds the
+// kernels: 62,496 x 5,120 takes 142 us, 6.8 TB/s (a plain copy of as many bytes 148); silu-mul, 31,248 x 13,824, 320 us, 6.8
+// TB/s; weight 15,360 x 5,120 36 us, 6.5 TB/s.  With 16-byte loads 153, 362 and 36 us; with checks and 64-bit products for
+// every load and single instead of packed fp32 products, twice the instructions, 168, 401 and 39 us.  Load and store hints
+// (evict first, no allocation in L1) measure the same or slower.
 #include "common.cuh"
 #include "quant.cuh"
 
@@ -21,32 +22,62 @@ namespace {
 
 constexpr int BLK = 128;
 
-// 8 bf16 values at x, `left` columns before the row's end, as bit patterns.  ALL: every one is in the row.  VEC: one 16-byte
-// load (K % 8 == 0, so they are all in the row or all past it); otherwise value by value, those past the end as zero
-template <bool VEC, bool ALL>
-__device__ __forceinline__ uint4 load8(const uint16_t* x, int64_t left) {
-  if constexpr (VEC) {
-    return ALL || left > 0 ? __ldg(reinterpret_cast<const uint4*>(x)) : make_uint4(0, 0, 0, 0);
-  } else {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t lo = 2 * i < left ? x[2 * i] : 0u;
-      const uint32_t hi = 2 * i + 1 < left ? x[2 * i + 1] : 0u;
-      w[i] = lo | (hi << 16);
-    }
-    return make_uint4(w[0], w[1], w[2], w[3]);
-  }
+// 16 bf16 values as bit patterns
+struct V16 {
+  uint32_t w[8];
+};
+
+// How a lane's 16 values of a block move: one 32-byte load and one 16-byte store, two 16-byte loads and 8-byte stores, or
+// value by value, every eighth from the lane's (its neighbours take the ones between: 999 x 5,130 in 25 us with 16 in a row)
+enum { SCALAR = 0, VEC16 = 1, VEC32 = 2 };
+template <int MODE>
+__device__ __forceinline__ int first_column() {
+  return (threadIdx.x & 7) * (MODE == SCALAR ? 1 : 16);
 }
 
-template <bool VEC, bool ALL>
-__device__ __forceinline__ void store8(uint8_t* q, int64_t left, uint2 v) {
-  if constexpr (VEC) {
-    if (ALL || left > 0) *reinterpret_cast<uint2*>(q) = v;
+// 16 values at x, `left` columns before the row's end; those past it as zero.  ALL: every one is in the row.  VEC32: K % 16 ==
+// 0, so all 16 are in the row or past it, VEC16: K % 8 == 0.
+template <int MODE, bool ALL>
+__device__ __forceinline__ V16 load16(const uint16_t* x, int64_t left) {
+  V16 v = {};
+  if constexpr (MODE == VEC32) {
+    if (ALL || left > 0)
+      asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                   : "=r"(v.w[0]), "=r"(v.w[1]), "=r"(v.w[2]), "=r"(v.w[3]), "=r"(v.w[4]), "=r"(v.w[5]), "=r"(v.w[6]), "=r"(v.w[7])
+                   : "l"(x));
+  } else if constexpr (MODE == VEC16) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (!ALL && left <= 8 * h) continue;
+      const uint4 a = __ldg(reinterpret_cast<const uint4*>(x) + h);
+      v.w[4 * h] = a.x;
+      v.w[4 * h + 1] = a.y;
+      v.w[4 * h + 2] = a.z;
+      v.w[4 * h + 3] = a.w;
+    }
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < left) q[i] = static_cast<uint8_t>((i < 4 ? v.x : v.y) >> (8 * (i & 3)));
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t lo = 16 * i < left ? x[16 * i] : 0u;
+      const uint32_t hi = 16 * i + 8 < left ? x[16 * i + 8] : 0u;
+      v.w[i] = lo | (hi << 16);
+    }
+  }
+  return v;
+}
+
+template <int MODE, bool ALL>
+__device__ __forceinline__ void store16(uint8_t* q, int64_t left, uint4 v) {
+  if constexpr (MODE == VEC32) {
+    if (ALL || left > 0) *reinterpret_cast<uint4*>(q) = v;
+  } else if constexpr (MODE == VEC16) {
+    if (ALL || left > 0) *reinterpret_cast<uint2*>(q) = make_uint2(v.x, v.y);
+    if (ALL || left > 8) *reinterpret_cast<uint2*>(q + 8) = make_uint2(v.z, v.w);
+  } else {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (8 * i < left) q[8 * i] = static_cast<uint8_t>(w[i >> 2] >> (8 * (i & 3)));
   }
 }
 
@@ -79,23 +110,28 @@ __device__ __forceinline__ uint32_t absmax2(uint32_t a, uint32_t b) {
   asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
-__device__ __forceinline__ uint32_t absmax_of(const uint4& v) { return absmax2(absmax2(v.x, v.y), absmax2(v.z, v.w)); }
-// the largest magnitude of a pair, as the bits of an fp32 (they order like the magnitudes, NaN above all)
+__device__ __forceinline__ uint32_t absmax_of(const V16& v) {
+  return absmax2(absmax2(absmax2(v.w[0], v.w[1]), absmax2(v.w[2], v.w[3])),
+                 absmax2(absmax2(v.w[4], v.w[5]), absmax2(v.w[6], v.w[7])));
+}
+// the bits of a bf16 magnitude as those of an fp32 (they order like the magnitudes, NaN above all)
 __device__ __forceinline__ uint32_t absmax_bits(uint32_t m2) { return fold16(m2 & 0x7FFF7FFFu) << 16; }
 
 // x * inv to e4m3, to nearest even; satfinite clamps to +-448 and keeps NaN
-__device__ __forceinline__ uint2 quant8(const F2 (&x)[4], float inv) {
-  uint32_t o[2];
+__device__ __forceinline__ uint4 quant16(const F2 (&x)[8], float inv) {
+  uint32_t o[4];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < 4; ++i) {
     const F2 a = mul2(x[2 * i], F2{inv, inv}), b = mul2(x[2 * i + 1], F2{inv, inv});
     o[i] = static_cast<uint32_t>(f32x2_to_e4m3x2(a.lo, a.hi)) | (static_cast<uint32_t>(f32x2_to_e4m3x2(b.lo, b.hi)) << 16);
   }
-  return make_uint2(o[0], o[1]);
+  return make_uint4(o[0], o[1], o[2], o[3]);
 }
-__device__ __forceinline__ uint2 quant8_bf16(const uint4& v, float inv) {
-  const F2 x[4] = {unpack2(v.x), unpack2(v.y), unpack2(v.z), unpack2(v.w)};
-  return quant8(x, inv);
+__device__ __forceinline__ uint4 quant16_bf16(const V16& v, float inv) {
+  F2 x[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = unpack2(v.w[i]);
+  return quant16(x, inv);
 }
 
 __device__ __forceinline__ float block_scale(uint32_t amax_bits, int div_mode) {
@@ -116,113 +152,112 @@ __device__ __forceinline__ F2 silu_mul2(F2 g, F2 u) {
   return mul2(mul2(g, r), u);
 }
 
-constexpr int U = 4;  // rows of a half-warp (two: 5.5 TB/s where four make 6.4)
+constexpr int U = 2, ROWS = 4 * U;  // rows of a lane (eight lanes hold a block), rows of a warp
 
-// Maxima of four values over the 16 lanes of a half-warp in 5 shuffles instead of 16: in each of the first two steps a lane
-// gives half of its values away and keeps the other half.  Lane hl is left with the maximum of value hl / 4.
-__device__ __forceinline__ uint32_t half_warp_max(const uint32_t (&v)[U], int hl) {
-  static_assert(U == 4, "two halving steps");
-  constexpr uint32_t ALL = 0xffffffffu;
-  const bool hi = hl & 8, odd = hl & 4;
-  uint32_t a = hi ? v[2] : v[0], b = hi ? v[3] : v[1];
-  a = max(a, __shfl_xor_sync(ALL, hi ? v[0] : v[2], 8));
-  b = max(b, __shfl_xor_sync(ALL, hi ? v[1] : v[3], 8));
-  uint32_t m = max(odd ? b : a, __shfl_xor_sync(ALL, odd ? a : b, 4));
-  m = max(m, __shfl_xor_sync(ALL, m, 2));
-  return max(m, __shfl_xor_sync(ALL, m, 1));
-}
-
-// A warp's unit: blocks of 2U consecutive rows at x (the lane's first row and column; SILU: up columns `K` further on), of
-// which this lane's half-warp has U.  `rows`, `left`: rows from the lane's first and columns from the lane's first to the end.
-template <bool VEC, bool SILU, bool ALL>
+// A warp's unit: one block of ROWS consecutive rows, at x the lane's first row and column (SILU: up columns K further on).
+// `rows`, `left`: rows from the lane's first and columns from the lane's first to the end.
+template <int MODE, bool SILU, bool ALL>
 __device__ __forceinline__ void quant_unit(const uint16_t* __restrict__ x, int64_t stride_x, int64_t K, int rows,
                                            int64_t left, uint8_t* __restrict__ q, float* __restrict__ s, int64_t s_row,
                                            int div_mode) {
-  const int hl = threadIdx.x & 15;
-  uint4 v[U], w[SILU ? U : 1];
+  static_assert(U == 2, "a lane's two rows");
+  constexpr uint32_t FULL = 0xffffffffu;
+  V16 v[U], w[SILU ? U : 1];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    v[u] = make_uint4(0, 0, 0, 0);
-    if (SILU) w[u] = make_uint4(0, 0, 0, 0);
+    v[u] = V16{};
+    if (SILU) w[u] = V16{};
     if (ALL || u < rows) {
-      v[u] = load8<VEC, ALL>(x, left);
-      if (SILU) w[u] = load8<VEC, ALL>(x + K, left);
+      v[u] = load16<MODE, ALL>(x, left);
+      if (SILU) w[u] = load16<MODE, ALL>(x + K, left);
     }
     x += stride_x;
   }
-  F2 y[SILU ? U : 1][4];
-  uint32_t amax[U];
+  // each lane is left with the largest magnitude of its row `mine` over the eight lanes, as fp32 bits
+  const bool mine = threadIdx.x & 4;
+  F2 y[SILU ? U : 1][8];
+  uint32_t amax;
+  if constexpr (SILU) {
+    float m[U];
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    if constexpr (SILU) {
-      const uint32_t g[4] = {v[u].x, v[u].y, v[u].z, v[u].w}, up[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
-      float m = 0.0f;
+    for (int u = 0; u < U; ++u) {
+      m[u] = 0.0f;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        y[u][e] = silu_mul2(unpack2(g[e]), unpack2(up[e]));
-        asm("max.NaN.abs.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(y[u][e].lo), "f"(y[u][e].hi));
+      for (int e = 0; e < 8; ++e) {
+        y[u][e] = silu_mul2(unpack2(v[u].w[e]), unpack2(w[u].w[e]));
+        asm("max.NaN.abs.f32 %0, %0, %1, %2;" : "+f"(m[u]) : "f"(y[u][e].lo), "f"(y[u][e].hi));
       }
-      amax[u] = __float_as_uint(m);
-    } else {
-      amax[u] = absmax_bits(absmax_of(v[u]));
     }
+    const uint32_t a = __float_as_uint(m[0]), b = __float_as_uint(m[1]);
+    amax = max(mine ? b : a, __shfl_xor_sync(FULL, mine ? a : b, 4));
+    amax = max(amax, __shfl_xor_sync(FULL, amax, 2));
+    amax = max(amax, __shfl_xor_sync(FULL, amax, 1));
+  } else {
+    // both rows' maxima as one pair of 16 bits
+    const uint32_t a = absmax_of(v[0]), b = absmax_of(v[1]);
+    uint32_t m2 = absmax2(__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632)) & 0x7FFF7FFFu;
+#pragma unroll
+    for (int o = 4; o; o >>= 1) m2 = __vmaxu2(m2, __shfl_xor_sync(FULL, m2, o));
+    amax = mine ? m2 & 0xFFFF0000u : m2 << 16;
   }
-  const float scale = block_scale(half_warp_max(amax, hl), div_mode);
+  const float scale = block_scale(amax, div_mode);
   const float inv = qdiv(1.0f, scale, div_mode);
-  if (hl % 4 == 0 && (ALL || hl / 4 < rows)) s[hl / 4 * s_row] = scale;
+  if ((threadIdx.x & 3) == 0 && (ALL || static_cast<int>(mine) < rows)) *(mine ? s + s_row : s) = scale;
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const float inv_u = __shfl_sync(0xffffffffu, inv, (threadIdx.x & 16) + u * 4);
+    const float inv_u = __shfl_sync(FULL, inv, (threadIdx.x & 24) + 4 * u);
     if (ALL || u < rows) {
       if constexpr (SILU)
-        store8<VEC, ALL>(q, left, quant8(y[u], inv_u));
+        store16<MODE, ALL>(q, left, quant16(y[u], inv_u));
       else
-        store8<VEC, ALL>(q, left, quant8_bf16(v[u], inv_u));
+        store16<MODE, ALL>(q, left, quant16_bf16(v[u], inv_u));
     }
     q += K;
   }
 }
 
-// rows x [rows, K] (SILU: [rows, 2K], gate | up) -> q [rows, K], s[row * s_row + j * s_blk].  A warp takes block j of 2U
-// consecutive rows, U per half-warp: their scales are then neighbours in the block-major scale tensor and leave in one
-// store, each division is made once per warp for 2U blocks, and the loads of a CTA's 4 warps run along the rows.
-template <bool VEC, bool SILU>
+// rows x [rows, K] (SILU: [rows, 2K], gate | up) -> q [rows, K], s[row * s_row + j * s_blk].  A warp takes block j of ROWS
+// consecutive rows: their scales are then neighbours in the block-major scale tensor and leave in one store, each division
+// is made once per warp for all of them, and the loads of a CTA's 4 warps run along the rows.  KB_inv: 2^64 / KB rounded up
+// (0 for KB = 1), so that a 64-bit product's upper half divides any 32-bit number by KB.
+template <int MODE, bool SILU>
 __global__ void __launch_bounds__(128) quant_blocks_kernel(const uint16_t* __restrict__ x, uint32_t rows, uint32_t units,
-                                                           uint32_t KB, int64_t K, int64_t stride_x,
+                                                           uint32_t KB, uint64_t KB_inv, int64_t K, int64_t stride_x,
                                                            uint8_t* __restrict__ q, float* __restrict__ s, int64_t s_row,
                                                            int64_t s_blk, int div_mode) {
   pdl_wait();
   pdl_launch();
   const uint32_t unit = blockIdx.x * 4u + (threadIdx.x >> 5);
   if (unit >= units) return;  // the whole warp
-  const uint32_t group = unit / KB, j = unit - group * KB;
-  const int64_t row0 = static_cast<int64_t>(group) * (2 * U) + (threadIdx.x & 16 ? U : 0);
-  const int64_t c = static_cast<int64_t>(j) * BLK + (threadIdx.x & 15) * 8;
+  const uint32_t group = KB_inv ? static_cast<uint32_t>(__umul64hi(KB_inv, unit)) : unit, j = unit - group * KB;
+  const int64_t row0 = static_cast<int64_t>(group) * ROWS + (threadIdx.x >> 3 & 3) * U;
+  const int64_t c = static_cast<int64_t>(j) * BLK + first_column<MODE>();
   x += row0 * stride_x + c;
   q += row0 * K + c;
   s += row0 * s_row + j * s_blk;
-  const bool all = (group + 1) * (2 * U) <= rows && (j + 1) * static_cast<int64_t>(BLK) <= K;
-  if (VEC && all)
-    quant_unit<VEC, SILU, VEC>(x, stride_x, K, U, 8, q, s, s_row, div_mode);
+  if (MODE != SCALAR && (group + 1) * ROWS <= rows && (j + 1) * static_cast<int64_t>(BLK) <= K)
+    quant_unit<MODE, SILU, MODE != SCALAR>(x, stride_x, K, U, 16, q, s, s_row, div_mode);
   else
-    quant_unit<VEC, SILU, false>(x, stride_x, K, static_cast<int>(rows) - static_cast<int>(row0), K - c, q, s, s_row,
-                                 div_mode);
+    quant_unit<MODE, SILU, false>(x, stride_x, K, static_cast<int>(rows) - static_cast<int>(row0), K - c, q, s, s_row,
+                                  div_mode);
 }
 
-// A CTA's tile: rows tile row r0 + 16 u of the lane at w (step_w elements apart), 8 columns each.  `rows`, `left` as above.
-template <bool VEC, bool ALL>
+// A CTA's tile: rows r0 + 32 u (u < 4) of the lane at w, step_w elements apart, 16 columns each.  `rows`, `left` as above.
+template <int MODE, bool ALL>
 __device__ __forceinline__ void quant_tile(const uint16_t* __restrict__ w, int64_t step_w, int64_t rows, int64_t left,
                                            uint8_t* __restrict__ q, int64_t step_q, float* __restrict__ s, int div_mode) {
   __shared__ uint32_t red[8];
   __shared__ float tile_scale[2];  // and its inverse
-  uint4 v[8];
+  V16 v[4];
   uint32_t m2 = 0;
 #pragma unroll
-  for (int u = 0; u < 8; ++u) {
-    v[u] = ALL || 16 * u < rows ? load8<VEC, ALL>(w, left) : make_uint4(0, 0, 0, 0);
-    m2 = absmax2(m2, absmax_of(v[u]));
+  for (int u = 0; u < 4; ++u) {
+    v[u] = V16{};
+    if (ALL || 32 * u < rows) v[u] = load16<MODE, ALL>(w, left);
     w += step_w;
   }
+#pragma unroll
+  for (int u = 0; u < 4; ++u) m2 = absmax2(m2, absmax_of(v[u]));
   const uint32_t wmax = __reduce_max_sync(0xffffffffu, absmax_bits(m2));
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = wmax;
   __syncthreads();
@@ -238,14 +273,14 @@ __device__ __forceinline__ void quant_tile(const uint16_t* __restrict__ w, int64
   const float inv = tile_scale[1];
   if (threadIdx.x == 0) *s = tile_scale[0];  // behind the barrier: ahead of it the others waited for it, 39.4 us for 36
 #pragma unroll
-  for (int u = 0; u < 8; ++u) {
-    if (ALL || 16 * u < rows) store8<VEC, ALL>(q, left, quant8_bf16(v[u], inv));
+  for (int u = 0; u < 4; ++u) {
+    if (ALL || 32 * u < rows) store16<MODE, ALL>(q, left, quant16_bf16(v[u], inv));
     q += step_q;
   }
 }
 
 // w [E, N, K] -> q [E, N, K] contiguous, s [E, NB, KB] contiguous: one CTA per tile
-template <bool VEC>
+template <int MODE>
 __global__ void __launch_bounds__(256) quant_weight_blocks_kernel(const uint16_t* __restrict__ w, int64_t N, int64_t K,
                                                                   int64_t stride_e, int64_t stride_n, uint32_t NB,
                                                                   uint32_t KB, uint8_t* __restrict__ q,
@@ -254,18 +289,24 @@ __global__ void __launch_bounds__(256) quant_weight_blocks_kernel(const uint16_t
   pdl_launch();
   const uint32_t tile = blockIdx.x;
   const uint32_t j = tile % KB, en = tile / KB, i = en % NB, e = en / NB;
-  const int64_t c = static_cast<int64_t>(j) * BLK + (threadIdx.x & 15) * 8;
-  const int64_t r0 = static_cast<int64_t>(i) * BLK + (threadIdx.x >> 4);
+  const int64_t c = static_cast<int64_t>(j) * BLK + first_column<MODE>();
+  const int64_t r0 = static_cast<int64_t>(i) * BLK + (threadIdx.x >> 3);
   w += e * stride_e + r0 * stride_n + c;
   q += (e * N + r0) * K + c;
   s += tile;
-  if (VEC && (i + 1) * static_cast<int64_t>(BLK) <= N && (j + 1) * static_cast<int64_t>(BLK) <= K)
-    quant_tile<VEC, VEC>(w, 16 * stride_n, BLK, 8, q, 16 * K, s, div_mode);
+  if (MODE != SCALAR && (i + 1) * static_cast<int64_t>(BLK) <= N && (j + 1) * static_cast<int64_t>(BLK) <= K)
+    quant_tile<MODE, MODE != SCALAR>(w, 32 * stride_n, BLK, 16, q, 32 * K, s, div_mode);
   else
-    quant_tile<VEC, false>(w, 16 * stride_n, N - r0, K - c, q, 16 * K, s, div_mode);
+    quant_tile<MODE, false>(w, 32 * stride_n, N - r0, K - c, q, 32 * K, s, div_mode);
 }
 
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+// how rows of K values at x (strides in elements) and bytes at q move
+int mode(const void* x, int64_t K, int64_t stride, int64_t stride2, const void* q) {
+  if (K % 16 == 0 && stride % 16 == 0 && stride2 % 16 == 0 && aligned(x, 32) && aligned(q, 16)) return VEC32;
+  return K % 8 == 0 && stride % 8 == 0 && stride2 % 8 == 0 && aligned(x, 16) && aligned(q, 8) ? VEC16 : SCALAR;
+}
 
 int bad_mode(int div_mode) { return div_mode != H3B_DIV_IEEE && div_mode != H3B_DIV_FULL; }
 
@@ -294,14 +335,14 @@ int quant_blocks(const char* what, const void* x, int64_t rows, int64_t K, int64
   if (stride_x < 0 || s_row < 0 || s_blk < 0) return fail(H3B_EINVAL, "%s: negative stride", what);
   const int64_t KB = (K + BLK - 1) / BLK;
   if (rows > ((1ll << 31) - 1) / KB) return fail(H3B_EUNSUPPORTED, "%s: 2^31 blocks or more", what);
-  const bool vec = K % 8 == 0 && stride_x % 8 == 0 && aligned(x, 16) && aligned(q, 8);
-  const auto units = static_cast<uint32_t>((rows + 2 * U - 1) / (2 * U) * KB);
+  const auto units = static_cast<uint32_t>((rows + ROWS - 1) / ROWS * KB);
   const unsigned grid = (units + 3) / 4;
-  const auto* xx = static_cast<const uint16_t*>(x);
-  auto* qq = static_cast<uint8_t*>(q);
-  return launch(what, vec ? quant_blocks_kernel<true, SILU> : quant_blocks_kernel<false, SILU>, grid, 128, st, xx,
-                static_cast<uint32_t>(rows), units, static_cast<uint32_t>(KB), K, stride_x, qq, s, s_row, s_blk,
-                static_cast<int>(div_mode));
+  const int m = mode(x, K, stride_x, 0, q);
+  const auto kernel = m == VEC32 ? quant_blocks_kernel<VEC32, SILU>
+                                 : (m == VEC16 ? quant_blocks_kernel<VEC16, SILU> : quant_blocks_kernel<SCALAR, SILU>);
+  return launch(what, kernel, grid, 128, st, static_cast<const uint16_t*>(x), static_cast<uint32_t>(rows), units,
+                static_cast<uint32_t>(KB), KB > 1 ? ~0ull / static_cast<uint64_t>(KB) + 1 : 0ull, K, stride_x,
+                static_cast<uint8_t*>(q), s, s_row, s_blk, static_cast<int>(div_mode));
 }
 
 }  // namespace
@@ -334,12 +375,11 @@ extern "C" int h3b_quant_weight_blocks_e4m3(const void* w, int64_t experts, int6
   if (stride_e < 0 || stride_n < 0) return fail(H3B_EINVAL, "quant_weight_blocks: negative stride");
   const int64_t NB = (n + BLK - 1) / BLK, KB = (k + BLK - 1) / BLK, most = (1ll << 31) - 1;
   if (NB > most / KB || experts > most / (NB * KB)) return fail(H3B_EUNSUPPORTED, "quant_weight_blocks: 2^31 tiles or more");
-  const bool vec = k % 8 == 0 && stride_n % 8 == 0 && stride_e % 8 == 0 && aligned(w, 16) && aligned(q, 8);
   const unsigned grid = static_cast<unsigned>(experts * NB * KB);
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const auto* ww = static_cast<const uint16_t*>(w);
-  auto* qq = static_cast<uint8_t*>(q);
-  return launch("quant_weight_blocks", vec ? quant_weight_blocks_kernel<true> : quant_weight_blocks_kernel<false>, grid,
-                256, st, ww, n, k, stride_e, stride_n, static_cast<uint32_t>(NB), static_cast<uint32_t>(KB), qq, scale,
-                static_cast<int>(div_mode));
+  const int m = mode(w, k, stride_n, stride_e, q);
+  const auto kernel = m == VEC32 ? quant_weight_blocks_kernel<VEC32>
+                                 : (m == VEC16 ? quant_weight_blocks_kernel<VEC16> : quant_weight_blocks_kernel<SCALAR>);
+  return launch("quant_weight_blocks", kernel, grid, 256, reinterpret_cast<cudaStream_t>(stream),
+                static_cast<const uint16_t*>(w), n, k, stride_e, stride_n, static_cast<uint32_t>(NB),
+                static_cast<uint32_t>(KB), static_cast<uint8_t*>(q), scale, static_cast<int>(div_mode));
 }

@@ -168,6 +168,23 @@ def test_quant_weight_blocks_strided(dev):
     assert torch.equal(codes(q), codes(rq)) and torch.equal(s, rs)
 
 
+@pytest.mark.parametrize("k", [256, 272, 264, 250])
+@pytest.mark.parametrize("m", [8, 13, 130])
+def test_quantisers_same_bits_for_any_alignment(dev, m, k):
+    """32-byte, 16-byte and single-value accesses: columns of a larger tensor that start at 0, 8, 16 and 1 values."""
+    base = (torch.randn(m, 2 * k, device=dev, generator=gen(m + k)) * 2).to(BF16)
+    want = ops.quant_blocks(base), ops.silu_mul_quant_blocks(base), ops.quant_weight_blocks(base)
+    for ld in (2 * k + 40, 2 * k + 48 - 2 * k % 16, 2 * k + 33):
+        big = torch.full((m + 1, ld), float("nan"), dtype=BF16, device=dev)
+        for first in (0, 8, 16, 1):
+            x = big[:m, first:first + 2 * k]
+            x.copy_(base)
+            got = ops.quant_blocks(x), ops.silu_mul_quant_blocks(x), ops.quant_weight_blocks(x)
+            for (q, s), (rq, rs) in zip(got, want):
+                assert torch.equal(s, rs) and torch.equal(codes(q), codes(rq))
+            big.fill_(float("nan"))
+
+
 @pytest.mark.parametrize("m,f,gain", [(1, 128, 1.0), (3, 100, 1.0), (17, 13824, 1.5), (40, 136, 30.0), (5, 77, 4.0)])
 def test_silu_mul_quant_blocks(dev, m, f, gain):
     x = (torch.randn(m, 2 * f, device=dev, generator=gen(f)) * gain).to(BF16)
