@@ -43,7 +43,8 @@ __device__ __forceinline__ V16 load16(const uint16_t* x, int64_t left) {
   if constexpr (MODE == VEC32) {
     if (ALL || left > 0)
       asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                   : "=r"(v.w[0]), "=r"(v.w[1]), "=r"(v.w[2]), "=r"(v.w[3]), "=r"(v.w[4]), "=r"(v.w[5]), "=r"(v.w[6]), "=r"(v.w[7])
+                   : "=r"(v.w[0]), "=r"(v.w[1]), "=r"(v.w[2]), "=r"(v.w[3]), "=r"(v.w[4]), "=r"(v.w[5]), "=r"(v.w[6]),
+                     "=r"(v.w[7])
                    : "l"(x));
   } else if constexpr (MODE == VEC16) {
 #pragma unroll

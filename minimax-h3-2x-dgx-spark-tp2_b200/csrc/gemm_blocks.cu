@@ -550,8 +550,10 @@ __global__ void __launch_bounds__(THREADS, 1)
 // ---------------------------------------------------------------------------------------------------------------
 namespace narrow {
 
-constexpr int EPI_WARPS = 8, EPI_THREADS = 32 * EPI_WARPS;
-constexpr int THREADS = 64 + EPI_THREADS;  // producer, MMA issuer, epilogue (4 row quarters x 2 token halves)
+// producer, MMA issuer, epilogue: 4 row quarters, and where a tile has more than 16 tokens 2 token halves (4 warps against 8:
+// 1 x 15,360 x 5,120 16.6 us for 16.7, 32 x 5,120 x 13,824 17.8 for 17.6, 64 x 15,360 x 5,120 22.5 for 21.2)
+__host__ __device__ constexpr int epi_warps(int nt) { return nt > 16 ? 8 : 4; }
+__host__ __device__ constexpr int threads(int nt) { return 64 + 32 * epi_warps(nt); }
 constexpr int CHUNK = 16;                  // K steps whose scales are staged together
 // as in the wide form: with 0, 48 rows over 64 experts of 4,096 x 5,120 take 118 us for 105 (10 and 40: 105).  Without parts
 // 1 x 5,120 x 5,120 takes 16.6 us for 8.2, 16 x 5,120 x 13,824 40 for 17
@@ -576,11 +578,12 @@ static_assert(tmem_fits(16) && tmem_fits(32) && tmem_fits(64), "TMEM columns");
 static_assert(STAGES * stage_bytes(64) >= 64 * BLK * 4 && smem(64) + 1024 <= 233472 / CTAS_PER_SM, "shared memory");
 
 template <int NT>
-__global__ void __launch_bounds__(THREADS, CTAS_PER_SM) kernel(const __grid_constant__ CUtensorMap tmA,
+__global__ void __launch_bounds__(threads(NT), CTAS_PER_SM) kernel(const __grid_constant__ CUtensorMap tmA,
                                                                    const __grid_constant__ CUtensorMap tmW,
                                                                    const __grid_constant__ Params p) {
   constexpr int STAGE_BYTES = stage_bytes(NT);
-  constexpr int MINE = NT / 2;  // tokens of an epilogue thread
+  constexpr int EPI_WARPS = epi_warps(NT), EPI_THREADS = 32 * EPI_WARPS;
+  constexpr int MINE = NT / (EPI_WARPS / 4);  // tokens of an epilogue thread
   constexpr uint32_t TMEM_COLS = NBUF * NT, IDESC = idesc_make(FMT_E4M3, FMT_E4M3, 0, 128, NT);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -739,19 +742,14 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) kernel(const __grid_cons
           }
           tc_fence_after();
           const uint32_t tcur = tmine + static_cast<uint32_t>(b * NT);
-          constexpr int W = MINE < 16 ? MINE : 16;
+          constexpr int W = 16;
+          static_assert(MINE % W == 0, "16 tokens at a time");
 #pragma unroll
           for (int c = 0; c < MINE; c += W) {
             uint32_t r[W];
-            if constexpr (W == 8)
-              tmem_ld8(tcur, r);
-            else
-              tmem_ld16(tcur + c, r);
+            tmem_ld16(tcur + c, r);
             tmem_ld_wait();
-            if constexpr (W >= 16)
-              reg_fence(r);
-            else
-              asm volatile("" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]));
+            reg_fence(r);
             if (c + W == MINE) {
               tc_fence_before();
               __syncwarp();
@@ -1014,7 +1012,7 @@ struct NarrowPlan : Plan {
     if (token_tiles > 65535)
       return fail(H3B_EUNSUPPORTED, "fp8_gemm_grouped: %lld row tiles of %d", (long long)token_tiles, NT);
     const void* kernel = reinterpret_cast<const void*>(narrow::kernel<NT>);
-    return pick_split(fits, kernel, kernel, narrow::THREADS, narrow::smem(NT), 1, narrow::CTAS_PER_SM, dev, tiles,
+    return pick_split(fits, kernel, kernel, narrow::threads(NT), narrow::smem(NT), 1, narrow::CTAS_PER_SM, dev, tiles,
                       p.num_kb, narrow::ROUND_COST, false, &split, &fit, &cost);
   }
   int go(Params& p, const Operands& o, const CUtensorMap& tmW, cudaStream_t st) {
@@ -1026,7 +1024,7 @@ struct NarrowPlan : Plan {
     if (rc) return rc;
     void* args[] = {&tmA, const_cast<CUtensorMap*>(&tmW), &p};
     return launch(reinterpret_cast<const void*>(narrow::kernel<NT>),
-                  dim3(static_cast<unsigned>(num_nb * split), static_cast<unsigned>(token_tiles), 1), narrow::THREADS,
+                  dim3(static_cast<unsigned>(num_nb * split), static_cast<unsigned>(token_tiles), 1), narrow::threads(NT),
                   narrow::smem(NT), split, args, st, nullptr);
   }
 };
