@@ -475,13 +475,13 @@ def _launch(ref: torch.Tensor, name: str, *args) -> None:
         _lib.call(name, *args, _stream(ref))
 
 
-def _unit_rows(t: torch.Tensor, dtype: torch.dtype, dims: int, what: str) -> tuple[int, ...]:
+def _unit_rows(t: torch.Tensor, dtype: torch.dtype, dims: int, what: str, arg: str = "") -> tuple[int, ...]:
     """The strides of a ``dims``-dimensional tensor of ``dtype`` whose rows are dense (unit innermost stride)."""
     if t.dtype != dtype:
-        raise TypeError(f"{what}: dtype {t.dtype}, expected {dtype}")
+        raise TypeError(f"{what}{arg}: dtype {t.dtype}, expected {dtype}")
     strides = t.stride()
     if len(strides) != dims or (strides[-1] != 1 and t.shape[-1] > 1):
-        raise ValueError(f"{what}: must have {dims} dimensions and unit innermost stride, got {tuple(t.shape)} with "
+        raise ValueError(f"{what}{arg}: must have {dims} dimensions and unit innermost stride, got {tuple(t.shape)} with "
                          f"strides {strides}")
     return strides
 
@@ -540,15 +540,15 @@ def quant_weight_blocks(w: torch.Tensor, *, div_mode: int = DIV_IEEE) -> tuple[t
 def _product_operands(a, w, sa, sb, others, out_dtype, out, what: str, dims: int):  # noqa: ANN001,ANN202
     """The operands that both block-scaled products share (w and sb of ``dims`` dimensions), checked.  Returns (m, n, k,
     row stride of a, strides of w, output, its row stride)."""
-    device = a.device
+    dev = a.get_device()    # ordinals first: six device objects cost a small call 1 us of 11
     for t in (a, w, sa, sb, out, *others):
-        if t is not None:
-            _need_cuda(t)
-            if t.device != device:
-                raise ValueError(f"{what}: tensors on {device} and {t.device}")
+        if t is not None and (dev < 0 or t.get_device() != dev):
+            _need_cuda(a, t)
+            if t.device != a.device:
+                raise ValueError(f"{what}: tensors on {a.device} and {t.device}")
     sa_t, sb_t = sa.dtype, sb.dtype
-    lda = _unit_rows(a, E4M3, 2, f"{what} a")[0]
-    w_strides = _unit_rows(w, E4M3, dims, f"{what} w")
+    lda = _unit_rows(a, E4M3, 2, what, " a")[0]
+    w_strides = _unit_rows(w, E4M3, dims, what, " w")
     m, k = a.shape
     *lead, n, k_w = w.shape
     if k_w != k or k < 16 or k % 16 or n < 1:
@@ -562,7 +562,7 @@ def _product_operands(a, w, sa, sb, others, out_dtype, out, what: str, dims: int
     if out is None:
         if out_dtype not in (torch.bfloat16, torch.float16):
             raise TypeError(f"{what}: out_dtype {out_dtype}, expected bf16 or f16")
-        out, ldy = torch.empty_strided((m, n), (n, 1), dtype=out_dtype, device=device), n
+        out, ldy = torch.empty_strided((m, n), (n, 1), dtype=out_dtype, device=a.device), n
     else:
         _dt(out, torch.bfloat16, torch.float16, what=f"{what} out")
         if tuple(out.shape) != (m, n) or (n > 1 and out.stride(1) != 1) or (m > 1 and out.stride(0) < n):
