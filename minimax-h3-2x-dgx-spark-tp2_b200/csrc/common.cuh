@@ -110,13 +110,18 @@ __device__ __forceinline__ bool mbar_wait_inline(uint32_t bar, uint32_t parity, 
 
 // ---- programmatic dependent launch: a kernel launched with the attribute may start while the one before it on its stream
 // ends.  pdl_wait returns once that kernel is complete and its writes are visible (at once without the attribute): no
-// global memory is touched before it, and every CTA calls it, so that completion carries over from kernel to kernel.
-// pdl_launch lets the next such kernel start; a kernel that allocates TMEM calls it when it has it, since the next one's
-// CTAs may take what is left.
+// global memory is touched before it, but for prefetches, which only bring lines into the coherent L2; and every CTA calls
+// it, so that completion carries over from kernel to kernel.  pdl_launch lets the next such kernel start; a kernel that
+// allocates TMEM calls it when it has it, since the next one's CTAs may take what is left.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 // ---- TMA (no multicast anywhere in this library) ----
+__device__ __forceinline__ void tma_prefetch_l2_3d(const CUtensorMap* m, int x, int y, int z) {
+  asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];" ::"l"(reinterpret_cast<uint64_t>(m)),
+               "r"(x), "r"(y), "r"(z)
+               : "memory");
+}
 __device__ __forceinline__ void tma_prefetch_desc(const CUtensorMap* m) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
 }

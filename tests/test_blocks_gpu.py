@@ -628,6 +628,31 @@ def test_back_to_back_launches_see_each_other(dev):
             assert torch.equal(g, w)
 
 
+@pytest.mark.parametrize("m", [1, 20, 64, 300])
+def test_weight_written_by_the_kernel_before(dev, m):
+    """The product's weight comes from the launch just ahead of it, at the same address every time."""
+    n, k = 2048, 2560
+    ws = [(torch.randn(n, k, device=dev, generator=gen(i)) * 0.05).to(BF16) for i in range(4)]
+    a, _, sa, _ = operands(m, 16, k)
+    want = []
+    for w in ws:
+        wq, sb = ops.quant_weight_blocks(w)
+        torch.cuda.synchronize()
+        want.append(ops.fp8_gemm_blocks(a, wq, sa, sb))
+        check_product(want[-1], a, wq, sa, sb)
+    packed = [ops.quant_weight_blocks(w) for w in ws]
+    held, held_s = torch.empty_like(packed[0][0]), torch.empty_like(packed[0][1])
+    torch.cuda.synchronize()
+    for i in range(40):
+        wq, sb = ops.quant_weight_blocks(ws[i % 4])
+        y = ops.fp8_gemm_blocks(a, wq, sa, sb)
+        del wq, sb
+        held.view(torch.uint8).copy_(packed[(i + 1) % 4][0].view(torch.uint8))
+        held_s.copy_(packed[(i + 1) % 4][1])
+        z = ops.fp8_gemm_blocks(a, held, sa, held_s)
+        assert torch.equal(y, want[i % 4]) and torch.equal(z, want[(i + 1) % 4])
+
+
 def test_two_streams_at_once(dev):
     a, w, sa, sb = operands(40, 1024, 2048, seed=3)
     b, v, sc, sd = operands(500, 1024, 2048, seed=4)
