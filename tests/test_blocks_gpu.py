@@ -322,6 +322,21 @@ def test_wide_product_bias_and_outputs(dev, m, n, k, out_dtype):
         assert bool((buf == 7).all())
 
 
+@pytest.mark.parametrize("first", [0, 1, 2, 4])
+@pytest.mark.parametrize("m,n,k", [*WIDE, (40, 300, 1024), (3, 129, 2048)])
+def test_outputs_of_every_alignment(dev, m, n, k, first):
+    """Rows that start 16, 8, 4 or 2 bytes aligned, all alike or in turn, and nothing written around them."""
+    a, w, sa, sb = operands(m, n, k, seed=4)
+    want = ops.fp8_gemm_blocks(a, w, sa, sb)
+    for ld in (n + 16 - n % 8, n + 12 - n % 4 + 4 * (n // 4 % 2), n + 10 - n % 2 + 2 * (n // 2 % 2), n + 9 + n % 2):
+        buf = torch.full((m + 2, ld), 7.0, dtype=BF16, device=dev)
+        out = buf[1:m + 1, first:first + n]
+        ops.fp8_gemm_blocks(a, w, sa, sb, out=out)
+        assert torch.equal(out, want)
+        out.fill_(7.0)
+        assert bool((buf == 7).all())
+
+
 @pytest.mark.parametrize("m,n,k", WIDE)
 def test_wide_product_is_exact_on_integers(dev, m, n, k):
     g = gen(m)
