@@ -66,6 +66,34 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
   return red[32];
 }
 
+// running abs-max of 8 bf16 values, kept as two packed 16-bit unsigned maxima
+__device__ __forceinline__ uint32_t absmax8(const uint4& v, uint32_t m2) {
+  m2 = __vmaxu2(m2, v.x & 0x7FFF7FFFu);
+  m2 = __vmaxu2(m2, v.y & 0x7FFF7FFFu);
+  m2 = __vmaxu2(m2, v.z & 0x7FFF7FFFu);
+  m2 = __vmaxu2(m2, v.w & 0x7FFF7FFFu);
+  return m2;
+}
+
+// 8 bf16 -> 8 e4m3 (one 8-byte word): x * inv, round to nearest even; satfinite clamps to +-448 exactly as the
+// reference's clamp does for every finite or infinite product, and keeps NaN
+__device__ __forceinline__ uint2 quant8(const uint4& v, float inv) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  uint32_t o[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint16_t a = f32x2_to_e4m3x2(lo_bf16(w[2 * i]) * inv, hi_bf16(w[2 * i]) * inv);
+    const uint16_t b = f32x2_to_e4m3x2(lo_bf16(w[2 * i + 1]) * inv, hi_bf16(w[2 * i + 1]) * inv);
+    o[i] = static_cast<uint32_t>(a) | (static_cast<uint32_t>(b) << 16);
+  }
+  return make_uint2(o[0], o[1]);
+}
+
+__device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
+  __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&h);
+}
+
 // the quant tail shared by every row kernel: row held as VPT x 8 bf16 per thread (vector i = tid + k*THREADS),
 // m2 = this thread's packed abs-max bits
 template <int THREADS, int VPT>
@@ -168,6 +196,14 @@ struct RmsArgs {
   int div_mode;
 };
 
+__device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = lo_bf16(w[i]);
+    f[2 * i + 1] = hi_bf16(w[i]);
+  }
+}
 __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
   return make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]),
                     pack_bf16x2(f[6], f[7]));
