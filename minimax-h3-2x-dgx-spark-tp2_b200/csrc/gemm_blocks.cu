@@ -21,9 +21,10 @@
 // epilogue warps (of both SMs) and back: 512 cycles of MMAs, then commit, TMEM reads under the additions and the arrival,
 // 1,200 more where the other SM is part of it, and 512 columns hold only two buffers.  Half as wide buffers, four of them:
 // 6.1 ms (twice the handshakes).  Sixteen epilogue warps of 64 columns: 7.7 ms.  Two additions per instruction (fma.rn.f32x2):
-// fewer cycles alone, more here.  Single CTAs have no cross-SM handshake, but read 48 KB a step and SM and meet the L2's limit
-// (about 12 TB/s) at the same speed.  Narrow: the weight's bytes, and at one row the start and end of a call: 1 x 15,360 x
-// 5,120 16.7 us (12.2 at copy speed), 1 x 5,120 x 5,120 8.1 (4.1).
+// fewer cycles alone, more here.  Single CTAs have no cross-SM handshake, but 48 KB a step and SM to fetch for 32, at
+// the same speed: 777 x 5,120 x 13,824 65 us; with a third of the loads left out 60, with most of the additions left out 60,
+// with both 56.  Spinning waits and L2 prefetches ahead of the ring gain nothing.  Narrow: the weight's bytes, and at one row
+// the start and end of a call: 1 x 15,360 x 5,120 16.4 us (12.2 at copy speed), 1 x 5,120 x 5,120 8.5 (4.1).
 //
 // Every wait is bounded (common.cuh); no TMA multicast.
 #include <atomic>
