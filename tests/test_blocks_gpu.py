@@ -684,6 +684,46 @@ def test_two_streams_at_once(dev):
     assert all(torch.equal(y, want[0]) for y in got[0]) and all(torch.equal(y, want[1]) for y in got[1])
 
 
+def test_threads_and_other_kernels_at_once(dev):
+    """Four host threads with a stream each: products of every form beside the per-token product and the attention."""
+    import threading
+
+    shapes = [(3, 1024, 2048), (40, 5120, 1024), (300, 9000, 512), (200, 5128, 2048)]
+    jobs = []
+    for m, n, k in shapes:
+        x = torch.randn(m, k, device=dev, generator=gen(m)).to(BF16)
+        w = ops.quant_weight_blocks((torch.randn(n, k, device=dev, generator=gen(n)) * 0.02).to(BF16))
+        q, s = ops.quant_blocks(x)
+        jobs.append((x, w, ops.fp8_gemm_blocks(q, w[0], s, w[1])))
+    a8 = torch.randn(512, 512, device=dev, generator=gen(1)).to(E4M3)
+    one = torch.ones(512, device=dev)
+    want8 = ops.fp8_gemm(a8, a8, one, one)
+    qkv = torch.randn(3, 512, 4, 128, device=dev, generator=gen(2)).to(BF16)
+    want_o = ops.flash_attn(qkv[0], qkv[1], qkv[2])
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(job):
+        x, w, want = job
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(30):
+                q, s = ops.quant_blocks(x)
+                y = ops.fp8_gemm_blocks(q, w[0], s, w[1])
+                y8 = ops.fp8_gemm(a8, a8, one, one)
+                o = ops.flash_attn(qkv[0], qkv[1], qkv[2])
+                torch.cuda.current_stream().synchronize()
+                if not (torch.equal(y, want) and torch.equal(y8, want8) and torch.equal(o, want_o)):
+                    wrong.append(x.shape)
+
+    threads = [threading.Thread(target=work, args=(j,)) for j in jobs]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join(60)
+    assert not wrong and not any(th.is_alive() for th in threads)
+    assert ops.device_status() == 0
+
+
 def test_torch_ops(dev):
     x = torch.randn(20, 512, device=dev, generator=gen(1)).to(BF16)
     q, s = torch.ops.h3b.quant_blocks(x)
