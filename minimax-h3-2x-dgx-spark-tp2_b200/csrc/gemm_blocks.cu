@@ -27,7 +27,9 @@
 // the start and end of a call: 1 x 15,360 x 5,120 16.4 us (12.2 at copy speed), 1 x 5,120 x 5,120 8.5 (4.1).
 //
 // Every wait is bounded (common.cuh); no TMA multicast.
+#include <algorithm>
 #include <atomic>
+#include <cmath>
 
 #include "common.cuh"
 
@@ -560,9 +562,11 @@ if (p.y_align == 16) {
             }
             uint4 out[2];
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-              out[h] = make_uint4(to_out2(v[8 * h], v[8 * h + 1], p.out_f16), to_out2(v[8 * h + 2], v[8 * h + 3], p.out_f16),
-                                  to_out2(v[8 * h + 4], v[8 * h + 5], p.out_f16), to_out2(v[8 * h + 6], v[8 * h + 7], p.out_f16));
+            for (int h = 0; h < 2; ++h) {
+              const float* f = v + 8 * h;
+              out[h] = make_uint4(to_out2(f[0], f[1], p.out_f16), to_out2(f[2], f[3], p.out_f16),
+                                  to_out2(f[4], f[5], p.out_f16), to_out2(f[6], f[7], p.out_f16));
+            }
             if (p.y_align == 16 && n + 16 <= p.N) {
               if (m0 + lane < walk.hi) {
                 uint4* dst = reinterpret_cast<uint4*>(p.y + (m0 + lane) * p.ldy + n);
@@ -1012,6 +1016,19 @@ struct Plan {
   double cost = 0;    // in steps
 };
 
+// tiles of `rows` rows to plan for.  Where there are several groups, each ends with part of a tile: half a tile more than the
+// rows make on average, sqrt(1 / 12) of one by chance, and that much is planned for, since a tile too many takes a whole
+// round: 500 rows in 4 groups of 1,024 x 8,192 21 us, without it 35 (where it is not needed K has fewer parts: 700 rows in 6
+// groups of 2,048 x 4,096 27 us for 22).  At least one for each group: 800 rows in 8 groups of
+// 5,120 x 5,120 58 us, without it 78
+int64_t expected_tiles(const Params& p, int64_t active, int64_t rows, int num_nb) {
+  const int64_t most = (p.T + active * (rows - 1)) / rows;  // exact for one group
+  if (p.experts == 1) return most * num_nb;
+  const double mean = static_cast<double>(p.T) / static_cast<double>(rows) + 0.5 * static_cast<double>(active);
+  const int64_t blocks = static_cast<int64_t>(std::ceil(mean + std::sqrt(static_cast<double>(active) / 12.0)));
+  return std::max(active, std::min(blocks, most)) * num_nb;
+}
+
 template <bool PAIR>
 struct WidePlan : Plan {
   static const void* whole() { return reinterpret_cast<const void*>(wide::kernel<PAIR, false>); }
@@ -1022,11 +1039,8 @@ struct WidePlan : Plan {
     constexpr int64_t ROWS = PAIR ? 2 * wide::BM : wide::BM;
     num_nb = static_cast<int>((p.N + wide::BN - 1) / wide::BN);
     tiles = (p.T + active * (ROWS - 1)) / ROWS * num_nb;
-    // to expect: T / ROWS and, where there are several groups, half a row block more for each
-    int64_t expected = p.experts == 1 ? tiles : (p.T + active * ROWS / 2) / ROWS * num_nb;
-    if (expected < 1) expected = 1;
-    return pick_split(fits, whole(), parts(), wide::THREADS, wide::SMEM, PAIR ? 2 : 1, 1, dev, expected, p.num_kb,
-                      wide::ROUND_COST, true, &split, &fit, &cost);
+    return pick_split(fits, whole(), parts(), wide::THREADS, wide::SMEM, PAIR ? 2 : 1, 1, dev,
+                      expected_tiles(p, active, ROWS, num_nb), p.num_kb, wide::ROUND_COST, true, &split, &fit, &cost);
   }
   int go(Params& p, const Operands& o, const CUtensorMap& tmW, cudaStream_t st) {
     p.num_nb = num_nb;
@@ -1063,8 +1077,8 @@ struct NarrowPlan : Plan {
     if (token_tiles > 65535)
       return fail(H3B_EUNSUPPORTED, "fp8_gemm_grouped: %lld row tiles of %d", (long long)token_tiles, NT);
     const void* kernel = reinterpret_cast<const void*>(narrow::kernel<NT>);
-    return pick_split(fits, kernel, kernel, narrow::threads(NT), narrow::smem(NT), 1, narrow::CTAS_PER_SM, dev, tiles,
-                      p.num_kb, narrow::ROUND_COST, false, &split, &fit, &cost);
+    return pick_split(fits, kernel, kernel, narrow::threads(NT), narrow::smem(NT), 1, narrow::CTAS_PER_SM, dev,
+                      expected_tiles(p, active, NT, num_nb), p.num_kb, narrow::ROUND_COST, false, &split, &fit, &cost);
   }
   int go(Params& p, const Operands& o, const CUtensorMap& tmW, cudaStream_t st) {
     p.num_nb = num_nb;
@@ -1141,7 +1155,8 @@ int gemm_blocks(const char* what, const Operands& o, cudaStream_t st) {
       narrow_nb > most / narrow::MAX_SPLIT)
     return fail(H3B_EUNSUPPORTED, "%s: 2^31 tiles or more", what);
   // Few rows a group: narrow.  Dense, 64 x 15,360 x 5,120: 20.7 us narrow, 24.4 wide; grouped, uneven groups of 20 rows
-  // in the mean (32 experts of 2,048 x 5,120): 75 and 102; of 38: 88 and 69, of 60: 101 and 69.
+  // in the mean (32 experts of 2,048 x 5,120): 75 and 102; of 38: 88 and 69, of 60: 101 and 69.  More rows: by cost, 300 rows
+  // in 4 groups of 1,024 x 4,096 12 and 15.
   if (mean > (o.E > 1 ? 32 : 64)) {
     WidePlan<true> pairs;
     WidePlan<false> singles;
@@ -1152,7 +1167,7 @@ int gemm_blocks(const char* what, const Operands& o, cudaStream_t st) {
     // x 27,648 x 5,120: 146 us, singles 152); single CTAs, with tiles of half the rows, fit small and ragged work better:
     // 777 x 5,120 x 13,824 in 65 us against 115
     const bool paired = pairs.cost <= SINGLE_STEP * singles.cost;
-    if (o.E == 1 && (o.T + 63) / 64 <= 65535) {
+    if ((o.T + active * 63) / 64 <= 65535) {
       NarrowPlan<64> few;
       rc = few.make(p, active, dev);
       if (rc) return rc;
