@@ -1163,9 +1163,9 @@ int gemm_blocks(const char* what, const Operands& o, cudaStream_t st) {
     rc = pairs.make(p, active, dev);
     if (!rc) rc = singles.make(p, active, dev);
     if (rc) return rc;
-    // CTA pairs read less (32 KB a step and SM instead of 48) and win by a few per cent where both take as many rounds (1,024
-    // x 27,648 x 5,120: 146 us, singles 152); single CTAs, with tiles of half the rows, fit small and ragged work better:
-    // 777 x 5,120 x 13,824 in 65 us against 115
+    // CTA pairs read less (32 KB a step and SM instead of 48), which counts at the power cap: 8,192 x 15,360 x 5,120 713 us in
+    // long runs, singles 746 (below the cap both 610); single CTAs, with tiles of half the rows, fit small and ragged work
+    // better: 777 x 5,120 x 13,824 65 us against 115, 1,500 rows in 8 groups of 2,048 x 5,120 31 against 52
     const bool paired = pairs.cost <= SINGLE_STEP * singles.cost;
     if ((o.T + active * 63) / 64 <= 65535) {
       NarrowPlan<64> few;
