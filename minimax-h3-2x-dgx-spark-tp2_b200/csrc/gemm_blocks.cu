@@ -368,22 +368,31 @@ __global__ void __launch_bounds__(THREADS, 1)
       bool have = false;
       float acc[128];
       int mb = 0, nb = 0;
-      for (int64_t t = first_tile; ok && walk.find(p, t, p.num_nb); t = next_tile(t)) {
+      int64_t m0 = 0, n0 = 0;  // the warp's first row and column
+      const float *sap = p.sa, *sbp = p.sb;
+      // the scales of the next two steps are on their way while a step is added; pairs ask for those of the next tile while one
+      // is stored (8,192 x 15,360 x 5,120 705 us for 717 in long runs; single CTAs, short of registers, lose 1 %)
+      float sa0 = 0.0f, sb0 = 0.0f, sa1 = 0.0f, sb1 = 0.0f;
+      auto find = [&](int64_t t) {
+        if (!walk.find(p, t, p.num_nb)) return false;
         coords(walk.r, walk.blocks, p.num_nb, mb, nb);
-        const int64_t m0 = walk.lo + (CTAS * mb + crank) * BM + sub * 32;  // the warp's first row
-        const int64_t n0 = static_cast<int64_t>(nb) * BN + half * 128;  // and first column
-        const bool row_ok = m0 + lane < walk.hi, col_ok = n0 < p.N;
-        const float* sap = p.sa + (row_ok ? m0 + lane : walk.lo) * p.sa_row;
-        const float* sbp = p.sb + walk.e * p.sb_exp + (col_ok ? n0 / BLK : 0) * p.sb_row;
-#pragma unroll
-        for (int i = 0; i < 128; ++i) acc[i] = 0.0f;
-        // the scales of the next two steps are on their way while a step is added
-        float sa0 = __ldg(sap + kb0 * p.sa_blk), sb0 = __ldg(sbp + kb0 * p.sb_blk);
-        float sa1 = 0.0f, sb1 = 0.0f;
+        m0 = walk.lo + (CTAS * mb + crank) * BM + sub * 32;
+        n0 = static_cast<int64_t>(nb) * BN + half * 128;
+        sap = p.sa + (m0 + lane < walk.hi ? m0 + lane : walk.lo) * p.sa_row;
+        sbp = p.sb + walk.e * p.sb_exp + (n0 < p.N ? n0 / BLK : 0) * p.sb_row;
+        sa0 = __ldg(sap + kb0 * p.sa_blk);
+        sb0 = __ldg(sbp + kb0 * p.sb_blk);
         if (kb0 + 1 < kb1) {
           sa1 = __ldg(sap + (kb0 + 1) * p.sa_blk);
           sb1 = __ldg(sbp + (kb0 + 1) * p.sb_blk);
         }
+        return true;
+      };
+      int64_t t = first_tile;
+      bool more = find(t);
+      while (more) {
+#pragma unroll
+        for (int i = 0; i < 128; ++i) acc[i] = 0.0f;
 #pragma unroll 1
         for (int kb = kb0; kb < kb1; ++kb, ++it) {
           const float s = sa0 * sb0;
@@ -438,13 +447,16 @@ __global__ void __launch_bounds__(THREADS, 1)
           have = true;
           break;
         }
+        const int64_t m_at = m0, n_at = n0, hi = walk.hi;
+        t = next_tile(t);
+        if constexpr (PAIR) more = find(t);
         if (p.bias != nullptr) {
 #pragma unroll
           for (int i = 0; i < 128; ++i)
-            if (n0 + i < p.N) acc[i] += __bfloat162float(p.bias[n0 + i]);
+            if (n_at + i < p.N) acc[i] += __bfloat162float(p.bias[n_at + i]);
         }
         // two halves of 64 columns through the warp's staging: 32 rows x 128 bytes in the 128-byte swizzle
-        const bool whole = p.tma_out && m0 + 32 <= walk.hi;
+        const bool whole = p.tma_out && m_at + 32 <= hi;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           if (p.tma_out && lane == 0) bulk_wait_read0();
@@ -455,23 +467,23 @@ __global__ void __launch_bounds__(THREADS, 1)
             stg[lane * 8 + (g ^ (lane & 7))] = make_uint4(to_out2(v[0], v[1], p.out_f16), to_out2(v[2], v[3], p.out_f16),
                                                           to_out2(v[4], v[5], p.out_f16), to_out2(v[6], v[7], p.out_f16));
           }
-          const int64_t nh = n0 + 64 * h;
+          const int64_t nh = n_at + 64 * h;
           // a TMA store ends at the map's edge rounded up to 16 bytes: slices across an odd edge leave row by row
           if (whole && (nh + 64 <= p.N || p.N % 8 == 0)) {
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0 && nh < p.N) {
-              tma_store_2d(&tmY, smem_u32(stg), static_cast<int32_t>(nh), static_cast<int32_t>(m0));
+              tma_store_2d(&tmY, smem_u32(stg), static_cast<int32_t>(nh), static_cast<int32_t>(m_at));
               bulk_commit();
             }
           } else {
             __syncwarp();
-if (p.y_align == 16) {
+            if (p.y_align == 16) {
 #pragma unroll 1
               for (int i = lane; i < 32 * 8; i += 32) {
                 const int r = i >> 3, g = i & 7;
-                const int64_t m = m0 + r, n = nh + 8 * g;
-                if (m >= walk.hi || n >= p.N) continue;
+                const int64_t m = m_at + r, n = nh + 8 * g;
+                if (m >= hi || n >= p.N) continue;
                 const uint4 val = stg[r * 8 + (g ^ (r & 7))];
                 uint16_t* dst = p.y + m * p.ldy + n;
                 if (n + 8 <= p.N) {
@@ -487,8 +499,8 @@ if (p.y_align == 16) {
               // a row per instruction, two columns a lane: from the row's first column, or from its second where only that one
               // is 4-byte aligned: 30,000 x 5,001 x 64 in 275 us (a value a lane: 308; eight values a lane, one by one: 546)
               const int left = static_cast<int>(p.N - nh < 64 ? p.N - nh : 64), c = 2 * lane;
-              const int rows = static_cast<int>(walk.hi - m0 < 32 ? walk.hi - m0 : 32);
-              uint16_t* dst = p.y + m0 * p.ldy + nh + c;
+              const int rows = static_cast<int>(hi - m_at < 32 ? hi - m_at : 32);
+              uint16_t* dst = p.y + m_at * p.ldy + nh + c;
 #pragma unroll 4
               for (int r = 0; r < rows; ++r, dst += p.ldy) {
                 const uint32_t val = reinterpret_cast<const uint32_t*>(stg)[(r * 8 + (lane >> 2 ^ (r & 7))) * 4 + (lane & 3)];
@@ -510,6 +522,7 @@ if (p.y_align == 16) {
             __syncwarp();
           }
         }
+        if constexpr (!PAIR) more = find(t);
       }
       if (p.tma_out && lane == 0) bulk_wait_all0();  // this warp's TMA stores are complete before the CTA leaves
       if constexpr (SPLIT) {
