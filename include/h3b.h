@@ -15,7 +15,8 @@
  *  - Return value: 0 (H3B_OK) or a negative h3b_status.  h3b_last_error() gives a one-line reason for the last
  *    failure of the calling thread.  Argument errors are detected on the host before anything is enqueued.
  *  - Device-side waits are bounded: a kernel whose pipeline stalls past H3B_WAIT_TIMEOUT_NS records
- *    H3B_ETIMEOUT in the per-device status word and returns; h3b_device_status() reads and clears it.
+ *    H3B_ETIMEOUT in the per-device status word and returns; h3b_device_status() reads and clears it.  Until then kernels
+ *    that wait return without their result.
  */
 #ifndef H3B_H_
 #define H3B_H_
@@ -232,9 +233,9 @@ H3B_API int h3b_fp8_gemm_blocks(const void* a, int64_t lda, const void* w, int64
 /* The same product grouped by expert: rows offsets[e] .. offsets[e+1] - 1 of a (and y) use w[e] (expert stride w_expert,
  * a multiple of 16) and sb[e] (expert stride sb_expert).  offsets: experts + 1 device integers (offsets_i64 != 0: int64,
  * else int32), non-decreasing, within [0, rows]; groups may be empty, and rows before the first or behind the last
- * bound are neither used nor written.  A group whose bounds break this is skipped and H3B_EINVAL recorded in the device
- * status word; rows that two other groups then claim hold the product of either or of neither.  The sizes are read on the
- * device only. */
+ * bound are neither used nor written.  A group whose bounds break this is skipped and H3B_EINVAL recorded for
+ * h3b_device_status; every other group is served, from the largest end of the groups before it on (so a row that two of
+ * them claim is the first one's), and no other call notices.  The sizes are read on the device only. */
 H3B_API int h3b_fp8_gemm_grouped(const void* a, int64_t lda, const void* w, int64_t w_expert, int64_t ldw,
                                  const float* sa, int64_t sa_row, int64_t sa_block, const float* sb, int64_t sb_expert,
                                  int64_t sb_row, int64_t sb_block, const void* offsets, int32_t offsets_i64, void* y,

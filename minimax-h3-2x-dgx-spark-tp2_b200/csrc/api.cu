@@ -43,8 +43,8 @@ int* device_status_word() {
   std::lock_guard<std::mutex> lock(g_status_mu);
   if (g_status[dev] == nullptr) {
     int* p = nullptr;
-    if (cudaMalloc(&p, sizeof(int)) != cudaSuccess) return nullptr;
-    if (cudaMemset(p, 0, sizeof(int)) != cudaSuccess) return nullptr;
+    if (cudaMalloc(&p, 2 * sizeof(int)) != cudaSuccess) return nullptr;
+    if (cudaMemset(p, 0, 2 * sizeof(int)) != cudaSuccess) return nullptr;
     g_status[dev] = p;
   }
   return g_status[dev];
@@ -123,11 +123,12 @@ int h3b_device_status(void) {
   if (w == nullptr) return h3b::fail(H3B_ECUDA, "no device status word");
   cudaError_t e = cudaDeviceSynchronize();
   if (e != cudaSuccess) return h3b::cuda_fail(e, "cudaDeviceSynchronize");
-  int v = 0;
-  e = cudaMemcpy(&v, w, sizeof(int), cudaMemcpyDeviceToHost);
+  int words[2] = {0, 0};
+  e = cudaMemcpy(words, w, sizeof(words), cudaMemcpyDeviceToHost);
   if (e != cudaSuccess) return h3b::cuda_fail(e, "reading the device status word");
+  const int v = words[0] != 0 ? words[0] : words[1];
   if (v != 0) {
-    cudaMemset(w, 0, sizeof(int));
+    cudaMemset(w, 0, sizeof(words));
     cudaDeviceSynchronize();
     h3b::set_error("device status word held %d (%s)", v, h3b_status_string(v));
   }

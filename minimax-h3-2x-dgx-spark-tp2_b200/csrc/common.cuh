@@ -19,7 +19,8 @@ namespace h3b {
 void set_error(const char* fmt, ...);
 int fail(int status, const char* fmt, ...);
 int cuda_fail(cudaError_t e, const char* what);
-// device status word of the current device (allocated once per device, zero-initialised)
+// device status words of the current device (allocated once per device, zero-initialised): the first one ends waits and keeps
+// kernels from starting, the second one holds what was wrong with a call's data and is looked at by the host only
 int* device_status_word();
 uint64_t wait_timeout_ns();
 // cuTensorMapEncodeTiled through the runtime's driver entry point (no -lcuda needed)
@@ -56,6 +57,9 @@ __device__ __forceinline__ bool status_bad(const WaitCtl& w) {
 }
 
 __device__ __forceinline__ void record_status(const WaitCtl& w, int code) { atomicCAS(w.status, 0, code); }
+// values in device memory (bounds, indices) that a call cannot use: nothing else stops for it.  Only with the words of
+// device_status_word().
+__device__ __forceinline__ void record_data_error(const WaitCtl& w, int code) { atomicCAS(w.status + 1, 0, code); }
 
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");

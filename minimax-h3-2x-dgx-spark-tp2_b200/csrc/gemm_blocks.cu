@@ -96,13 +96,15 @@ __device__ __forceinline__ void store4(const Params& p, int64_t at, int64_t n, f
 
 // Walk over the row tiles of the groups in order.  `before`: tiles of the experts below e0.  find() places tile t
 // (non-decreasing over calls) with the whole warp: 32 experts' bounds per step and a shuffle scan.  A group whose bounds
-// are not 0 <= lo <= hi <= T has no tiles, and `bad` is set (recorded by the caller once its cluster is done, so that
-// the CTAs of a cluster never disagree on whether to start).
+// are not 0 <= lo <= hi <= T has no tiles, and `bad` is set.  From then on a group's rows start at `reach` at the earliest, the
+// largest end before it: no row is in two groups, so that there are never more tiles than the launch has counted on.
+// (While no bound is bad they are in order, and lo is `reach`.)
 template <int ROWS>
 struct Walk {
   int e0 = 0;
   int64_t before = 0;
-  bool bad = false;
+  bool bad = false;    // the same for the whole warp
+  int reach = 0;       // of the experts below e0
   int e;               // the tile found: expert, its rows [lo, hi), row blocks and the tile's index within the expert
   int64_t lo, hi;
   int blocks, r;
@@ -110,17 +112,30 @@ struct Walk {
     const int lane = threadIdx.x & 31;
     while (e0 < p.experts) {
       int64_t l = 0, h = 0;
+      bool wrong = false;
       if (e0 + lane < p.experts) {
         if (p.offsets == nullptr) {
           h = p.T;
         } else {
           l = group_bound(p, e0 + lane);
           h = group_bound(p, e0 + lane + 1);
-          if (l < 0 || h < l || h > p.T) {
-            l = h = 0;
-            bad = true;
-          }
+          wrong = l < 0 || h < l || h > p.T;
+          if (wrong) l = h = 0;
         }
+      }
+      const int last = static_cast<int>(h);  // at most T, which is below 2^31
+      bad |= __any_sync(0xffffffffu, wrong);
+      if (bad) {
+        int most = max(last, reach);  // of the groups up to this lane's, then before it
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int up = __shfl_up_sync(0xffffffffu, most, o);
+          if (lane >= o) most = max(most, up);
+        }
+        most = __shfl_up_sync(0xffffffffu, most, 1);
+        if (lane == 0) most = reach;
+        l = l > most ? l : most;
+        h = h > l ? h : l;
       }
       const int mine = static_cast<int>((h - l + ROWS - 1) / ROWS);
       int64_t sum = static_cast<int64_t>(mine) * per_block;
@@ -142,6 +157,7 @@ struct Walk {
       }
       before += total;
       e0 += 32;
+      reach = max(reach, __reduce_max_sync(0xffffffffu, last));
     }
     return false;
   }
@@ -247,8 +263,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   const uint32_t tmem_base = *tmem_slot;
   const bool start = cluster_flag(smem_u32(start_flag));  // of the cluster's first CTA
   const int first_tile = static_cast<int>(cluster_id_x()), tile_step = static_cast<int>(cluster_count_x());
-  // parts of K: a cluster takes one tile.  Bounds that overlap make more tiles than the launch counted on: those are left
-  // out (the last find only looks for the bad bounds that there must be)
+  // parts of K: a cluster takes one tile, and the last find only looks for bad bounds
   auto next_tile = [&](int64_t t) { return SPLIT ? INT64_MAX : t + tile_step; };
   Walk<CTAS * BM> walk;
   bool ok = true;  // no wait of this thread's role has given up
@@ -615,7 +630,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     else
       tmem_dealloc(tmem_base, 512);
   }
-  if (walk.bad) record_status(p.wc, H3B_EINVAL);
+  if (walk.bad && lane == 0) record_data_error(p.wc, H3B_EINVAL);
 }
 
 }  // namespace wide
@@ -684,7 +699,7 @@ __global__ void __launch_bounds__(threads(NT), CTAS_PER_SM) kernel(const __grid_
   Walk<NT> walk;
   const bool found = walk.find(p, blockIdx.y, 1);  // the same for every CTA of the cluster
   if (!found) {
-    if (walk.bad) record_status(p.wc, H3B_EINVAL);
+    if (walk.bad && lane == 0) record_data_error(p.wc, H3B_EINVAL);
     return;
   }
   const int64_t t0 = walk.lo + static_cast<int64_t>(walk.r) * NT;  // the tile's first row of a
@@ -899,7 +914,7 @@ __global__ void __launch_bounds__(threads(NT), CTAS_PER_SM) kernel(const __grid_
   cluster_sync();  // the other CTAs have read this CTA's sums (and its start flag)
   tc_fence_after();
   if (warp == 1) tmem_dealloc(tmem_base, TMEM_COLS);
-  if (walk.bad) record_status(p.wc, H3B_EINVAL);
+  if (walk.bad && lane == 0) record_data_error(p.wc, H3B_EINVAL);
 }
 
 }  // namespace narrow

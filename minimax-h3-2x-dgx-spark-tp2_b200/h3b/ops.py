@@ -598,8 +598,8 @@ def fp8_gemm_grouped(a: torch.Tensor, w: torch.Tensor, sa: torch.Tensor, sb: tor
     times w[e] of w [E, N, K], with sb [E, ceil(N/128), ceil(K/128)].  ``offsets``: E + 1 int32 or int64 values on the
     device, non-decreasing within [0, T]; the host never reads them.  Groups may be empty.  Rows before offsets[0] and
     from offsets[E] on are not written (a fresh output is uninitialised there).  Bounds out of order or out of range
-    skip their group and record H3B_EINVAL in the device status word (``device_status``); rows that two of the other
-    groups then claim are undefined."""
+    skip their group and record H3B_EINVAL (``device_status``); every other group is served, from the largest end of the
+    groups before it on, and no other call notices."""
     wide = offsets.dtype == torch.int64
     if not wide and offsets.dtype != torch.int32:
         raise TypeError(f"fp8_gemm_grouped: offsets {offsets.dtype}, expected int32 or int64")
