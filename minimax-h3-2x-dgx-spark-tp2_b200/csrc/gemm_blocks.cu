@@ -171,6 +171,14 @@ __device__ __forceinline__ bool cluster_flag(uint32_t flag_smem) {
   return v != 0;
 }
 
+// A wait of this CTA has given up, so its sums are not whole: every CTA of the cluster (they add each other's) is told, and
+// stores nothing.  `flag`: cleared before the cluster's first barrier, read behind one that follows this.
+__device__ __forceinline__ void give_up(uint32_t flag_smem, int ctas) {
+  for (int r = 0; r < ctas; ++r)
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(mapa_shared(flag_smem, static_cast<uint32_t>(r))), "r"(1u)
+                 : "memory");
+}
+
 // ---------------------------------------------------------------------------------------------------------------
 // wide: 256 x 256 tiles by CTA pairs or 128 x 256 by single CTAs, running sums in registers
 // ---------------------------------------------------------------------------------------------------------------
@@ -214,11 +222,12 @@ __global__ void __launch_bounds__(THREADS, 1)
   constexpr int STAGES = stages(PAIR), STAGE_BYTES = stage_bytes(PAIR), CTAS = PAIR ? 2 : 1;
   constexpr uint32_t IDESC = idesc_make(FMT_E4M3, FMT_E4M3, 0, CTAS * BM, BN);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + RING_BYTES);
-  // bars: full[STAGES], used[STAGES], tempty[2], done; then the TMEM address and the start flag.  used[s]: the MMAs of
+  // bars: full[STAGES], used[STAGES], tempty[2], done; then the TMEM address, the start and give-up flags.  used[s]: the MMAs of
   // the step in stage s are complete, which frees the stage for the producer and hands the step's accumulator to the
   // epilogue (one commit per step for both)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 3);
   uint32_t* start_flag = tmem_slot + 1;
+  volatile uint32_t* gave_up = start_flag + 1;
   uint8_t* staging = smem + RING_BYTES + 1024;
   const uint32_t smem0 = smem_u32(smem), bar0 = smem_u32(bars);
   auto full_bar = [&](int s) { return bar0 + 8u * s; };
@@ -255,7 +264,10 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
   }
   pdl_wait();
-  if (threadIdx.x == 0) *start_flag = status_bad(p.wc) ? 0u : 1u;
+  if (threadIdx.x == 0) {
+    *start_flag = status_bad(p.wc) ? 0u : 1u;
+    *gave_up = 0u;
+  }
   tc_fence_before();
   cluster_sync();
   tc_fence_after();
@@ -546,6 +558,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         // stores: 100 x 5,120 x 5,120 in 23.4 us for 15.9, the reads of other CTAs' memory want lanes side by side)
         __syncthreads();  // every load has landed and every MMA has read the ring
         float4* sums = reinterpret_cast<float4*>(smem);
+        if (!ok && lane == 0) give_up(smem_u32(start_flag + 1), CTAS * p.split);
         if (have) {
 #pragma unroll
           for (int i = 0; i < 32; ++i)
@@ -555,7 +568,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         __syncwarp();
         cluster_sync();
         const int64_t m0 = walk.lo + (CTAS * mb + crank) * BM + sub * 32;  // the warp's first row
-        if (have && m0 < walk.hi) {
+        if (have && *gave_up == 0u && m0 < walk.hi) {
           for (int g = part + half * p.split; g < BN / 16; g += 2 * p.split) {
             const int64_t n = static_cast<int64_t>(nb) * BN + 16 * g;
             if (n >= p.N) break;
@@ -679,13 +692,14 @@ __global__ void __launch_bounds__(threads(NT), CTAS_PER_SM) kernel(const __grid_
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE_BYTES);
-  // bars: full[STAGES], used[STAGES], tempty[NBUF], done; then the TMEM address and the start flag.  used[s]: the MMAs of
-  // the step in stage s are complete, for the producer and for the epilogue.
+  // bars: full[STAGES], used[STAGES], tempty[NBUF], done; then the TMEM address, the start and give-up flags.  used[s]: the
+  // MMAs of the step in stage s are complete, for the producer and for the epilogue.
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + NBUF + 1);
   uint32_t* start_flag = tmem_slot + 1;
+  volatile uint32_t* gave_up = start_flag + 1;
   float* scales = reinterpret_cast<float*>(smem + STAGES * STAGE_BYTES + 256);  // [2][CHUNK][NT]
   float* sums = reinterpret_cast<float*>(smem);                                 // [NT][128] once the ring is idle
-  static_assert(8 * (2 * STAGES + NBUF + 1) + 8 <= 256, "barrier area");
+  static_assert(8 * (2 * STAGES + NBUF + 1) + 12 <= 256, "barrier area");
   const uint32_t smem0 = smem_u32(smem), bar0 = smem_u32(bars);
   auto full_bar = [&](int s) { return bar0 + 8u * s; };
   auto used_bar = [&](int s) { return bar0 + 8u * (STAGES + s); };
@@ -727,7 +741,10 @@ __global__ void __launch_bounds__(threads(NT), CTAS_PER_SM) kernel(const __grid_
     tmem_relinquish();
   }
   pdl_wait();
-  if (threadIdx.x == 0) *start_flag = status_bad(p.wc) ? 0u : 1u;
+  if (threadIdx.x == 0) {
+    *start_flag = status_bad(p.wc) ? 0u : 1u;
+    *gave_up = 0u;
+  }
   tc_fence_before();
   cluster_sync();
   tc_fence_after();
@@ -862,6 +879,7 @@ __global__ void __launch_bounds__(threads(NT), CTAS_PER_SM) kernel(const __grid_
           }
         }
       }
+      if (!ok && lane == 0) give_up(smem_u32(start_flag + 1), split);
     }
   }
   __syncwarp();
@@ -873,7 +891,7 @@ __global__ void __launch_bounds__(threads(NT), CTAS_PER_SM) kernel(const __grid_
   const float bias = epi && p.bias != nullptr && n < p.N ? __bfloat162float(p.bias[n]) : 0.0f;
   const int tokens = static_cast<int>(walk.hi - t0 < NT ? walk.hi - t0 : NT);
   if (split == 1) {
-    if (epi && start && n < p.N) {
+    if (epi && start && *gave_up == 0u && n < p.N) {
 #pragma unroll
       for (int i = 0; i < MINE; ++i)
         if (first + i < tokens) p.y[(t0 + first + i) * p.ldy + n] = to_out(acc[i] + bias, p.out_f16);
@@ -889,7 +907,7 @@ __global__ void __launch_bounds__(threads(NT), CTAS_PER_SM) kernel(const __grid_
     // loads are on their way before the first is added (64 x 5,120 x 5,120: 11.4 us, one load at a time 12.8); added in the
     // order of K
     const int64_t n4 = static_cast<int64_t>(nb) * BLK + 4 * lane;
-    if (epi && start && n4 < p.N) {
+    if (epi && start && *gave_up == 0u && n4 < p.N) {
       for (int i = crank + split * (warp - 2); i < tokens; i += EPI_WARPS * split) {
         float part[MAX_SPLIT][4];
 #pragma unroll
