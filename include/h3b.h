@@ -190,7 +190,7 @@ H3B_API int h3b_fp8_gemm(const void* a, int64_t lda, const void* w, int64_t ldw,
  * y[m, n] = bf16(x[m, n] + gate[indices[m], n] * o) in fp32 with separate rounding of the product and the sum.
  * x, gate, y: bf16 row-major with leading dimensions ldx, ld_gate, ldy (multiples of 8, 16-byte aligned);
  * indices: int64 [M] (row of gate for each token, in [0, gate_rows); a row whose index is outside leaves y
- * untouched and records H3B_EINVAL in the device status word). */
+ * untouched and records H3B_EINVAL for h3b_device_status; no other row and no other call notices). */
 H3B_API int h3b_fp8_gemm_gate(const void* a, int64_t lda, const void* w, int64_t ldw, const float* sa,
                               const float* sb, const void* bias, const void* x, int64_t ldx, const void* gate,
                               int64_t ld_gate, int64_t gate_rows, const int64_t* indices, void* y, int64_t ldy,

@@ -647,7 +647,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MODE == MODE_STD ? T
                 if (mr >= p.M || g >= granules) continue;
                 const int64_t gi = __ldg(p.gidx + mr);
                 if (gi < 0 || gi >= p.gate_rows) {
-                  record_status(p.wc, H3B_EINVAL);
+                  record_data_error(p.wc, H3B_EINVAL);
                   continue;
                 }
                 const int64_t col = nbk + g * 8;

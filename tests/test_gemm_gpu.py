@@ -395,3 +395,28 @@ def test_strided_output_rows_keep_their_gaps(dev):
     assert same_bits(y.cpu(), ref.cpu())
     assert bool((buf[:, N:] == 7.0).all())
     assert ops.device_status() == 0
+
+
+def test_gate_index_out_of_range_stops_no_other_call(dev):
+    """A bad index is its row's alone: the others and the calls behind it, with the status still unread, are served."""
+    from h3b import _lib
+    M, N, K = 20000, 512, 256
+    g = torch.Generator(device=dev).manual_seed(4)
+    a = torch.randint(-2, 3, (M, K), device=dev, generator=g).to(E4M3)
+    w = torch.randint(-2, 3, (N, K), device=dev, generator=g).to(E4M3)
+    sa, sb = torch.full((M,), 1e-3, device=dev), torch.full((N,), 1e-3, device=dev)
+    x = torch.randn(M, N, device=dev, generator=g).to(BF16)
+    gate = torch.ones(2, N, device=dev, dtype=BF16)
+    idx = torch.zeros(M, device=dev, dtype=torch.int64)
+    want = ops.fp8_gemm_gate(a, w, sa, sb, x, gate, idx)
+    plain = ops.fp8_gemm(a, w, sa, sb)
+    assert ops.device_status() == 0
+    idx[5], idx[M - 1] = -1, 2
+    want[5], want[M - 1] = 5.0, 5.0
+    for _ in range(2):
+        y = torch.full((M, N), 5.0, device=dev, dtype=BF16)
+        ops.fp8_gemm_gate(a, w, sa, sb, x, gate, idx, out=y)
+        assert torch.equal(y, want)
+        assert torch.equal(ops.fp8_gemm(a, w, sa, sb), plain)
+    assert ops.device_status() == _lib.H3B_EINVAL
+    assert ops.device_status() == 0
