@@ -209,7 +209,8 @@ H3B_API int h3b_quant_blocks_e4m3(const void* x, int64_t rows, int64_t cols, int
                                   int64_t scale_row, int64_t scale_block, int32_t div_mode, h3b_stream_t stream);
 
 /* x [rows, 2d] bf16 (gate columns, then up columns): the block quant of h = gate / (1 + exp(-gate)) * up, with h in fp32
- * (h is not rounded to bf16 on the way, unlike h3b_silu_mul_quant_e4m3).  q [rows, d], scales as above. */
+ * (h is not rounded to bf16 on the way, unlike h3b_silu_mul_quant_e4m3), within (5 + 0.75 |gate|) * 2^-23 of its size for
+ * normal gates and h.  q [rows, d], scales as above. */
 H3B_API int h3b_silu_mul_quant_blocks_e4m3(const void* x, int64_t rows, int64_t d, int64_t stride_x, void* q,
                                            float* scale, int64_t scale_row, int64_t scale_block, int32_t div_mode,
                                            h3b_stream_t stream);

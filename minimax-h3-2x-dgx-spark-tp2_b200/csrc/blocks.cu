@@ -141,7 +141,8 @@ __device__ __forceinline__ float block_scale(uint32_t amax_bits, int div_mode) {
 
 // silu(g) * u = g / (1 + 2^(-g log2 e)) * u in fp32, not rounded before the quant: one rounding, to e4m3.  The argument's
 // rounding counts |g| * 0.75, ex2.approx 2, rcp.approx 1 and the other four steps half a unit each: within (5 + 0.75 |g|) *
-// 2^-23 in all, against the 2^-4 of e4m3.  Below g = -87 the reciprocal, under 2^-126, is flushed and silu is 0.
+// 2^-23 in all (g and the result being normal numbers), against the 2^-4 of e4m3.  For gates down to -87: below, the reciprocal
+// is under 2^-126 and flushed.
 __device__ __forceinline__ F2 silu_mul2(F2 g, F2 u) {
   constexpr float NEG_LOG2E = -1.4426950408889634f;
   F2 e = mul2(g, F2{NEG_LOG2E, NEG_LOG2E});
@@ -153,7 +154,57 @@ __device__ __forceinline__ F2 silu_mul2(F2 g, F2 u) {
   return mul2(mul2(g, r), u);
 }
 
+// The same for any gate: below -87, silu(g) = g 2^(g log2 e) to 2^-125, computed 2^64 times as large and scaled back behind the
+// product with u, which may be 2^127.  Within the same bound.  (From g = -131 on the exponential is flushed even so, and |h| is
+// under 10^-16: a code of 0.)  -inf gives NaN, as g / (1 + exp(-g)) does.
+__device__ __forceinline__ float silu_mul_far(float g, float u) {
+  const F2 near = silu_mul2(F2{g, g}, F2{u, u});
+  float e = fmaf(g, 1.4426950408889634f, 64.0f);
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e));
+  return g < -87.0f ? g * e * u * 5.421010862427522e-20f : near.lo;
+}
+
 constexpr int U = 2, ROWS = 4 * U;  // rows of a lane (eight lanes hold a block), rows of a warp
+
+// Whether a warp's gates have one below -87 and its ups one of 2^90 or more (or either a NaN).  With smaller ups silu(g) * u of
+// such a gate is under 2^-29: a code of 0 by either way, and nothing to the block's maximum.  As unsigned 16-bit patterns the
+// negative gates lie above the others, in the order of their magnitudes.
+__device__ __forceinline__ bool any_far(const V16 (&gate)[U], const V16 (&up)[U]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = __vimax3_u16x2(m, gate[0].w[i], gate[1].w[i]);
+  if (!__any_sync(0xffffffffu, fold16(m) > 0xC2AEu)) return false;
+  m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = __vimax3_u16x2(m, up[0].w[i] & 0x7FFF7FFFu, up[1].w[i] & 0x7FFF7FFFu);
+  return __any_sync(0xffffffffu, fold16(m) >= 0x6C80u);
+}
+
+// A unit (as below) with such values, which hardly ever come up: value by value, `step` columns apart, each twice, in few
+// registers.  A call, so that the other units' code stays as it is: with both in one loop 31,248 x 13,824 takes 6 % longer
+// (nothing measurable so; 2 ms for 300 us if every unit has such values).
+__device__ __noinline__ void far_unit(const uint16_t* x, int64_t stride_x, int64_t K, int rows, int64_t left, int step,
+                                      uint8_t* q, float* s, int64_t s_row, int div_mode) {
+  auto value = [&](int i) {
+    return silu_mul_far(bf16_bits_to_f32(x[step * i]), bf16_bits_to_f32(x[K + step * i]));
+  };
+#pragma unroll 1
+  for (int u = 0; u < U; ++u, x += stride_x, q += K, s += s_row) {
+    float m = 0.0f;
+#pragma unroll 1
+    for (int i = 0; i < 16 && u < rows && step * i < left; ++i)
+      asm("max.NaN.abs.f32 %0, %0, %1, 0f00000000;" : "+f"(m) : "f"(value(i)));
+    uint32_t amax = __float_as_uint(m);
+#pragma unroll
+    for (int o = 4; o; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    const float scale = block_scale(amax, div_mode);
+    const float inv = qdiv(1.0f, scale, div_mode);
+    if ((threadIdx.x & 7) == 0 && u < rows) *s = scale;
+#pragma unroll 1
+    for (int i = 0; i < 16 && u < rows && step * i < left; ++i)
+      q[step * i] = static_cast<uint8_t>(f32x2_to_e4m3x2(value(i) * inv, 0.0f));
+  }
+}
 
 // A warp's unit: one block of ROWS consecutive rows, at x the lane's first row and column (SILU: up columns K further on).
 // `rows`, `left`: rows from the lane's first and columns from the lane's first to the end.
@@ -173,6 +224,10 @@ __device__ __forceinline__ void quant_unit(const uint16_t* __restrict__ x, int64
       if (SILU) w[u] = load16<MODE, ALL>(x + K, left);
     }
     x += stride_x;
+  }
+  if constexpr (SILU) {
+    if (any_far(v, w))  // the whole warp
+      return far_unit(x - U * stride_x, stride_x, K, rows, left, MODE == SCALAR ? 8 : 1, q, s, s_row, div_mode);
   }
   // each lane is left with the largest magnitude of its row `mine` over the eight lanes, as fp32 bits
   const bool mine = threadIdx.x & 4;
