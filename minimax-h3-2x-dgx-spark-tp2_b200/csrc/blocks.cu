@@ -36,13 +36,14 @@ __device__ __forceinline__ int first_column() {
 }
 
 // 16 values at x, `left` columns before the row's end; those past it as zero.  ALL: every one is in the row.  VEC32: K % 16 ==
-// 0, so all 16 are in the row or past it, VEC16: K % 8 == 0.
+// 0, so all 16 are in the row or past it, VEC16: K % 8 == 0.  Plain loads: the kernel ahead may write x while this one already
+// runs (common.cuh).
 template <int MODE, bool ALL>
 __device__ __forceinline__ V16 load16(const uint16_t* x, int64_t left) {
   V16 v = {};
   if constexpr (MODE == VEC32) {
     if (ALL || left > 0)
-      asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+      asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                    : "=r"(v.w[0]), "=r"(v.w[1]), "=r"(v.w[2]), "=r"(v.w[3]), "=r"(v.w[4]), "=r"(v.w[5]), "=r"(v.w[6]),
                      "=r"(v.w[7])
                    : "l"(x));
@@ -50,7 +51,7 @@ __device__ __forceinline__ V16 load16(const uint16_t* x, int64_t left) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       if (!ALL && left <= 8 * h) continue;
-      const uint4 a = __ldg(reinterpret_cast<const uint4*>(x) + h);
+      const uint4 a = reinterpret_cast<const uint4*>(x)[h];
       v.w[4 * h] = a.x;
       v.w[4 * h + 1] = a.y;
       v.w[4 * h + 2] = a.z;
@@ -209,7 +210,7 @@ __device__ __noinline__ void far_unit(const uint16_t* x, int64_t stride_x, int64
 // A warp's unit: one block of ROWS consecutive rows, at x the lane's first row and column (SILU: up columns K further on).
 // `rows`, `left`: rows from the lane's first and columns from the lane's first to the end.
 template <int MODE, bool SILU, bool ALL>
-__device__ __forceinline__ void quant_unit(const uint16_t* __restrict__ x, int64_t stride_x, int64_t K, int rows,
+__device__ __forceinline__ void quant_unit(const uint16_t* x, int64_t stride_x, int64_t K, int rows,
                                            int64_t left, uint8_t* __restrict__ q, float* __restrict__ s, int64_t s_row,
                                            int div_mode) {
   static_assert(U == 2, "a lane's two rows");
@@ -277,7 +278,7 @@ __device__ __forceinline__ void quant_unit(const uint16_t* __restrict__ x, int64
 // is made once per warp for all of them, and the loads of a CTA's 4 warps run along the rows.  KB_inv: 2^64 / KB rounded up
 // (0 for KB = 1), so that a 64-bit product's upper half divides any 32-bit number by KB.
 template <int MODE, bool SILU>
-__global__ void __launch_bounds__(128) quant_blocks_kernel(const uint16_t* __restrict__ x, uint32_t rows, uint32_t units,
+__global__ void __launch_bounds__(128) quant_blocks_kernel(const uint16_t* x, uint32_t rows, uint32_t units,
                                                            uint32_t KB, uint64_t KB_inv, int64_t K, int64_t stride_x,
                                                            uint8_t* __restrict__ q, float* __restrict__ s, int64_t s_row,
                                                            int64_t s_blk, int div_mode) {
@@ -300,7 +301,7 @@ __global__ void __launch_bounds__(128) quant_blocks_kernel(const uint16_t* __res
 
 // A CTA's tile: rows r0 + 32 u (u < 4) of the lane at w, step_w elements apart, 16 columns each.  `rows`, `left` as above.
 template <int MODE, bool ALL>
-__device__ __forceinline__ void quant_tile(const uint16_t* __restrict__ w, int64_t step_w, int64_t rows, int64_t left,
+__device__ __forceinline__ void quant_tile(const uint16_t* w, int64_t step_w, int64_t rows, int64_t left,
                                            uint8_t* __restrict__ q, int64_t step_q, float* __restrict__ s, int div_mode) {
   __shared__ uint32_t red[8];
   __shared__ float tile_scale[2];  // and its inverse
@@ -337,7 +338,7 @@ __device__ __forceinline__ void quant_tile(const uint16_t* __restrict__ w, int64
 
 // w [E, N, K] -> q [E, N, K] contiguous, s [E, NB, KB] contiguous: one CTA per tile
 template <int MODE>
-__global__ void __launch_bounds__(256) quant_weight_blocks_kernel(const uint16_t* __restrict__ w, int64_t N, int64_t K,
+__global__ void __launch_bounds__(256) quant_weight_blocks_kernel(const uint16_t* w, int64_t N, int64_t K,
                                                                   int64_t stride_e, int64_t stride_n, uint32_t NB,
                                                                   uint32_t KB, uint8_t* __restrict__ q,
                                                                   float* __restrict__ s, int div_mode) {

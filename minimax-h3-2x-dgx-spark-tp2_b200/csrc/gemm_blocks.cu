@@ -61,8 +61,8 @@ struct Params {
 };
 
 __device__ __forceinline__ int64_t group_bound(const Params& p, int e) {
-  return p.off64 ? __ldg(static_cast<const int64_t*>(p.offsets) + e)
-                 : static_cast<int64_t>(__ldg(static_cast<const int32_t*>(p.offsets) + e));
+  return p.off64 ? static_cast<const int64_t*>(p.offsets)[e]
+                 : static_cast<int64_t>(static_cast<const int32_t*>(p.offsets)[e]);
 }
 
 __device__ __forceinline__ uint16_t to_out(float v, int f16) {
@@ -407,11 +407,11 @@ __global__ void __launch_bounds__(THREADS, 1)
         n0 = static_cast<int64_t>(nb) * BN + half * 128;
         sap = p.sa + (m0 + lane < walk.hi ? m0 + lane : walk.lo) * p.sa_row;
         sbp = p.sb + walk.e * p.sb_exp + (n0 < p.N ? n0 / BLK : 0) * p.sb_row;
-        sa0 = __ldg(sap + kb0 * p.sa_blk);
-        sb0 = __ldg(sbp + kb0 * p.sb_blk);
+        sa0 = sap[kb0 * p.sa_blk];
+        sb0 = sbp[kb0 * p.sb_blk];
         if (kb0 + 1 < kb1) {
-          sa1 = __ldg(sap + (kb0 + 1) * p.sa_blk);
-          sb1 = __ldg(sbp + (kb0 + 1) * p.sb_blk);
+          sa1 = sap[(kb0 + 1) * p.sa_blk];
+          sb1 = sbp[(kb0 + 1) * p.sb_blk];
         }
         return true;
       };
@@ -426,8 +426,8 @@ __global__ void __launch_bounds__(THREADS, 1)
           sa0 = sa1;
           sb0 = sb1;
           if (kb + 2 < kb1) {
-            sa1 = __ldg(sap + (kb + 2) * p.sa_blk);
-            sb1 = __ldg(sbp + (kb + 2) * p.sb_blk);
+            sa1 = sap[(kb + 2) * p.sa_blk];
+            sb1 = sbp[(kb + 2) * p.sb_blk];
           }
           const int b = it & 1;
           if (!__all_sync(0xffffffffu, mbar_wait_inline(used_bar(stage), phase, p.wc))) {
@@ -827,7 +827,7 @@ __global__ void __launch_bounds__(threads(NT), CTAS_PER_SM) kernel(const __grid_
         for (int i = 0; i < PER; ++i) {
           const int v = tid + EPI_THREADS * i, k = kb + v / NT, tok = v % NT;
           next[i] = (k < kb1 && t0 + tok < walk.hi)
-                        ? __ldg(p.sa + (t0 + tok) * p.sa_row + k * p.sa_blk) * __ldg(sbp + k * p.sb_blk)
+                        ? p.sa[(t0 + tok) * p.sa_row + k * p.sa_blk] * sbp[k * p.sb_blk]
                         : 0.0f;
         }
       };
