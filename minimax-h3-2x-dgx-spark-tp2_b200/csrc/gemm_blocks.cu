@@ -1120,8 +1120,6 @@ struct NarrowPlan : Plan {
     num_nb = static_cast<int>((p.N + BLK - 1) / BLK);
     token_tiles = (p.T + active * (NT - 1)) / NT;
     tiles = token_tiles * num_nb;
-    if (token_tiles > 65535)
-      return fail(H3B_EUNSUPPORTED, "fp8_gemm_grouped: %lld row tiles of %d", (long long)token_tiles, NT);
     const void* kernel = reinterpret_cast<const void*>(narrow::kernel<NT>);
     return pick_split(fits, kernel, kernel, narrow::threads(NT), narrow::smem(NT), 1, narrow::CTAS_PER_SM, dev,
                       expected_tiles(p, active, NT, num_nb), p.num_kb, narrow::ROUND_COST, false, &split, &fit, &cost);
@@ -1138,6 +1136,9 @@ struct NarrowPlan : Plan {
                   narrow::smem(NT), split, args, st, nullptr);
   }
 };
+
+// whether the narrow form's grid, whose second axis counts row tiles, has a place for all that there can be
+bool narrow_serves(const Params& p, int64_t active, int rows) { return (p.T + active * (rows - 1)) / rows <= 65535; }
 
 template <int NT>
 int launch_narrow(Params& p, const Operands& o, const CUtensorMap& tmW, int64_t active, int dev, cudaStream_t st) {
@@ -1203,7 +1204,7 @@ int gemm_blocks(const char* what, const Operands& o, cudaStream_t st) {
   // Few rows a group: narrow.  Dense, 64 x 15,360 x 5,120: 20.7 us narrow, 24.4 wide; grouped, uneven groups of 20 rows
   // in the mean (32 experts of 2,048 x 5,120): 75 and 102; of 38: 88 and 69, of 60: 101 and 69.  More rows: by cost, 300 rows
   // in 4 groups of 1,024 x 4,096 12 and 15.
-  if (mean > (o.E > 1 ? 32 : 64)) {
+  if (mean > (o.E > 1 ? 32 : 64) || !narrow_serves(p, active, mean <= 16 ? 16 : 32)) {
     WidePlan<true> pairs;
     WidePlan<false> singles;
     rc = pairs.make(p, active, dev);
@@ -1213,7 +1214,7 @@ int gemm_blocks(const char* what, const Operands& o, cudaStream_t st) {
     // long runs, singles 746 (below the cap both 610); single CTAs, with tiles of half the rows, fit small and ragged work
     // better: 777 x 5,120 x 13,824 65 us against 115, 1,500 rows in 8 groups of 2,048 x 5,120 31 against 52
     const bool paired = pairs.cost <= SINGLE_STEP * singles.cost;
-    if ((o.T + active * 63) / 64 <= 65535) {
+    if (narrow_serves(p, active, 64)) {
       NarrowPlan<64> few;
       rc = few.make(p, active, dev);
       if (rc) return rc;
