@@ -44,7 +44,12 @@ int* device_status_word() {
   if (g_status[dev] == nullptr) {
     int* p = nullptr;
     if (cudaMalloc(&p, 2 * sizeof(int)) != cudaSuccess) return nullptr;
-    if (cudaMemset(p, 0, 2 * sizeof(int)) != cudaSuccess) return nullptr;
+    // the zeros must be there before a kernel of any stream reads them: the memset is asynchronous, and streams that do not
+    // block with the default one do not wait for it
+    if (cudaMemset(p, 0, 2 * sizeof(int)) != cudaSuccess || cudaStreamSynchronize(cudaStreamLegacy) != cudaSuccess) {
+      cudaFree(p);
+      return nullptr;
+    }
     g_status[dev] = p;
   }
   return g_status[dev];

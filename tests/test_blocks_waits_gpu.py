@@ -1,4 +1,7 @@
 """The block-scaled products beside a device wait that runs out: what is in an output is right or was there before."""
+import subprocess
+import sys
+
 import pytest
 import torch
 from test_blocks_gpu import operands
@@ -36,3 +39,21 @@ def test_products_beside_a_wait_that_gives_up(dev, m, n, k):
     assert bool((outs[-1] == 7).all())
     assert ops.device_status() == 0
     assert torch.equal(ops.fp8_gemm_blocks(a, w, sa, sb), want)
+
+
+def test_first_call_of_a_process_on_a_side_stream(dev):
+    """The status words are allocated by the first product, whose kernel may not see them before they are zero."""
+    code = ("import sys; sys.path[:0] = %r\n"
+            "import torch\n"
+            "from h3b import ops\n"
+            "a = torch.ones(40, 256, device='cuda').to(torch.float8_e4m3fn)\n"
+            "s, t = torch.ones(40, 2, device='cuda'), torch.ones(1, 2, device='cuda')\n"
+            "torch.cuda.synchronize()\n"
+            "with torch.cuda.stream(torch.cuda.Stream()):\n"
+            "    y = ops.fp8_gemm_blocks(a, a, s, t)\n"
+            "    z = ops.fp8_gemm_blocks(a, a, s, t)\n"
+            "torch.cuda.synchronize()\n"
+            "assert bool((y == 256).all()) and bool((z == 256).all())\n"
+            "assert ops.device_status() == 0\n") % sys.path
+    run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0, run.stderr
