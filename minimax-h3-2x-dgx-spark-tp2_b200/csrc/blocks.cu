@@ -10,10 +10,10 @@
 // written once.
 //
 // Long runs sit at the power cap, where each instruction costs clock, so their number counts although memory bounds the
-// kernels: 62,496 x 5,120 takes 142 us, 6.8 TB/s (a plain copy of as many bytes 148); silu-mul, 31,248 x 13,824, 320 us, 6.8
-// TB/s; weight 15,360 x 5,120 36 us, 6.5 TB/s.  With 16-byte loads 153, 362 and 36 us; with checks and 64-bit products for
-// every load and single instead of packed fp32 products, twice the instructions, 168, 401 and 39 us.  Load and store hints
-// (evict first, no allocation in L1) measure the same or slower.
+// kernels: 62,496 x 5,120 takes 142 us, 6.8 TB/s (a plain copy of as many bytes 148); silu-mul, 31,248 x 13,824, 320 to 332 us
+// on different days, 6.6 to 6.8 TB/s; weight 15,360 x 5,120 36 us, 6.5 TB/s.  With 16-byte loads 153, 362 and 36 us; with
+// checks and 64-bit products for every load and single instead of packed fp32 products, twice the instructions, 168, 401 and
+// 39 us.  Load and store hints (evict first, no allocation in L1) measure the same or slower.
 #include "common.cuh"
 #include "quant.cuh"
 

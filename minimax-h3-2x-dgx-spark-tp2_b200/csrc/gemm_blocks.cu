@@ -26,6 +26,10 @@
 // with both 56.  Spinning waits and L2 prefetches ahead of the ring gain nothing.  Narrow: the weight's bytes, and at one row
 // the start and end of a call: 1 x 15,360 x 5,120 16.4 us (12.2 at copy speed), 1 x 5,120 x 5,120 8.5 (4.1).
 //
+// Spills (-Xptxas -v: 132 bytes in the pair form, 116 in the single one, 16 in narrow<64>) lie outside the loop over K: the local
+// loads and stores of a launch are the same for twice the K.  With K in parts pairs have five loads and a store a step and
+// epilogue warp in it, single CTAs two and one.
+//
 // Every wait is bounded (common.cuh); no TMA multicast.
 #include <algorithm>
 #include <atomic>
@@ -815,11 +819,11 @@ __global__ void __launch_bounds__(threads(NT), CTAS_PER_SM) kernel(const __grid_
         }
       }
     } else {
-      // ---------------- epilogue: thread = weight row and half of the tokens ----------------
+      // ---------------- epilogue: thread = weight row and MINE of the tokens ----------------
       const int sub = warp & 3, half = (warp - 2) >> 2, tid = threadIdx.x - 64;
       const uint32_t tmine = tmem_base + (static_cast<uint32_t>(sub * 32) << 16) + static_cast<uint32_t>(half * MINE);
       const float* sbp = p.sb + walk.e * p.sb_exp + nb * p.sb_row;
-      // sa * sb of a chunk of steps for the tile's tokens; thread tid holds values tid, tid + 256, ... of [CHUNK][NT]
+      // sa * sb of a chunk of steps for the tile's tokens; thread tid holds values tid, tid + EPI_THREADS, ... of [CHUNK][NT]
       constexpr int PER = CHUNK * NT / EPI_THREADS;
       float next[PER];
       auto fetch = [&](int kb) {

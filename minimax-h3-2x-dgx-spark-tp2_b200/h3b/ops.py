@@ -596,7 +596,7 @@ def fp8_gemm_grouped(a: torch.Tensor, w: torch.Tensor, sa: torch.Tensor, sb: tor
                      out_dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None) -> torch.Tensor:
     """``fp8_gemm_blocks`` with one weight per expert: rows offsets[e] .. offsets[e+1] of a [T, K] (sorted by expert)
     times w[e] of w [E, N, K], with sb [E, ceil(N/128), ceil(K/128)].  ``offsets``: E + 1 int32 or int64 values on the
-    device, non-decreasing within [0, T]; the host never reads them.  Groups may be empty.  Rows before offsets[0] and
+    device, non-decreasing within [0, T]; the host never reads them.  No bias.  Groups may be empty.  Rows before offsets[0] and
     from offsets[E] on are not written (a fresh output is uninitialised there).  Bounds out of order or out of range
     skip their group and record H3B_EINVAL (``device_status``); every other group is served, from the largest end of the
     groups before it on, and no other call notices."""
