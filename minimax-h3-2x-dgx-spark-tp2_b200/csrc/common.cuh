@@ -116,8 +116,8 @@ __device__ __forceinline__ bool mbar_wait_inline(uint32_t bar, uint32_t parity, 
 // ends.  pdl_wait returns once that kernel is complete and its writes are visible (at once without the attribute): no
 // global memory is touched before it, but for prefetches, which only bring lines into the coherent L2; and every CTA calls
 // it, so that completion carries over from kernel to kernel.  What the kernel before may write is not constant for this one's
-// lifetime, so it is read by plain loads, without __ldg, .nc or const __restrict__.  pdl_launch lets the next such kernel start; a kernel that
-// allocates TMEM calls it when it has it, since the next one's CTAs may take what is left.
+// lifetime, so it is read by plain loads, without __ldg, .nc or const __restrict__.  pdl_launch lets the next such kernel
+// start; a kernel that allocates TMEM calls it when it has it, since the next one's CTAs may take what is left.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
